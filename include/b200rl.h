@@ -655,6 +655,93 @@ int b200rl_permute_rows(float* data, int ld, int n_rows, const int32_t* perm, un
 int b200rl_shuffle_rows(float* data, int ld, int n_rows, unsigned long long column_mask, uint32_t* rng_state_host, int32_t* perm_host, int32_t* perm, void* scratch,
                         size_t scratch_bytes, void* sent, void* used, b200rl_stream_t copy_stream, b200rl_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Residual networks in 16-bit types: dense layers whose epilogue carries bias, activation and residual, the norms around a block fused with
+ * its gate and residual scale, and dropout whose mask is drawn from a counter and never stored. (No counterpart in the reference, whose
+ * networks are chains of fp32 layers.)
+ *   - `type` is the type of the matrices that are passed as void*; biases, norm weights and all parameter gradients are fp32, so that they
+ *     lie in the arenas of b200rl_adam_step; 16-bit weights are the caller's copy of its fp32 master weights.
+ *   - row pitches (ld*) are in elements of `type` and at least the row's length; rows may start at any address that is a multiple of the
+ *     element's size (fastest: 16-byte aligned rows). A pitch of a matrix with at most one row is not looked at.
+ *   - sums, statistics and products are held in fp32 and rounded to `type` once, when they are stored.
+ *   - calls that share scratch, a workspace or a gradient must be ordered on one stream (or by events).
+ *   - an output may not overlap an input, unless a comment below allows it.
+ * ------------------------------------------------------------------------------------------------------- */
+#define B200RL_TYPE_FLOAT32 0
+#define B200RL_TYPE_BFLOAT16 1
+#define B200RL_TYPE_FLOAT16 2
+/* further activations, for the entry points of this section alone: x Phi(x) with the normal distribution function Phi, and x sigmoid(x) */
+#define B200RL_ACT_GELU 5
+#define B200RL_ACT_SILU 6
+#define B200RL_NORM_NONE 0
+#define B200RL_NORM_LAYER 1     /* (x - mean) / sqrt(variance + epsilon), the variance over the row's `dim` elements */
+#define B200RL_NORM_RMS 2       /* x / sqrt(mean of squares + epsilon) */
+#define B200RL_NORM_MAX_DIM 8192
+
+/* pre = x W^T + bias; y = residual + scale act(pre). type: bfloat16 or float16 (b200rl_dense_forward is the fp32 layer). W [output, input],
+ * x [batch, input], bias fp32 [output] or NULL, residual [batch, output] or NULL (none added); pre [batch, output] or NULL receives the
+ * pre-activations, which the backward pass needs for every activation but the identity. y may be residual itself (same pitch).
+ * workspace: ..._workspace_bytes of the same operands (16-byte aligned; 0 bytes and NULL for most calls): split-k partial sums of small
+ * batches, and copies of operands whose rows are not 16-byte aligned. Nothing in it is kept between calls. */
+size_t b200rl_dense_residual_forward_workspace_bytes(const void* W, int ldw, const void* x, int ldx, int batch, int input_dim, int output_dim);
+int b200rl_dense_residual_forward(int type, const void* W, int ldw, const float* bias, const void* x, int ldx, const void* residual, int ldr, float scale,
+                                  void* pre, int ldpre, void* y, int ldy, int batch, int input_dim, int output_dim, int activation,
+                                  void* workspace, size_t workspace_bytes, b200rl_stream_t stream);
+
+/* d_pre = scale act'(pre) d_y, all [rows, cols] of `type` (bfloat16 or float16); pre may be NULL for the identity. d_pre may be d_y or pre
+ * itself (same pitch). The gradient of the residual is d_y as it is. */
+int b200rl_dense_residual_backward_activation(int type, const void* pre, int ldpre, const void* d_y, int ldd, float scale, void* d_pre, int lddp, int rows,
+                                              int cols, int activation, b200rl_stream_t stream);
+
+/* d_in = act'(pre_in) (d_pre W + add): the gradient of the layer's input, with `add` [batch, input] (or NULL) the gradient that reaches the same
+ * input by another way (a residual around this layer) and, for an activation_in other than the identity, on through the activation whose
+ * pre-activations pre_in [batch, input] were (the previous layer's d_pre; NULL for the identity). d_in may be add or pre_in itself (same pitch). */
+size_t b200rl_dense_residual_backward_input_workspace_bytes(const void* W, int ldw, const void* d_pre, int ldd, int batch, int input_dim, int output_dim);
+int b200rl_dense_residual_backward_input(int type, const void* W, int ldw, const void* d_pre, int ldd, const void* add, int lda, const void* pre_in, int ldp,
+                                         int activation_in, void* d_in, int ldi, int batch, int input_dim, int output_dim, void* workspace,
+                                         size_t workspace_bytes, b200rl_stream_t stream);
+
+/* d_W [output, input] (dense rows) = d_pre^T x and d_bias [output] = column sums of d_pre (either may be NULL), both fp32; accumulate != 0 adds onto
+ * what they hold, 0 overwrites it. Every sum has a fixed order. The batch is summed in fp32 pieces of 512 rows, so that long batches lose nothing
+ * to the tensor core's accumulator, which truncates. */
+size_t b200rl_dense_residual_backward_weights_workspace_bytes(const void* x, int ldx, const void* d_pre, int ldd, int batch, int input_dim, int output_dim);
+int b200rl_dense_residual_backward_weights(int type, const void* x, int ldx, const void* d_pre, int ldd, float* d_W, float* d_bias, int accumulate, int batch,
+                                           int input_dim, int output_dim, void* workspace, size_t workspace_bytes, b200rl_stream_t stream);
+
+/* One pass between two blocks of a residual network, every type:
+ *   u = post(branch), out = residual + scale gate u, normed = pre(out)        (the norm behind the block, gate and scale; the norm in front of the next)
+ * with post, pre one of B200RL_NORM_*, each norm followed by its weight and bias (fp32 [dim], NULL: 1 and 0). gate [ceil(rows / gate_rows), dim] of
+ * `type` or NULL (1): row r takes gate row r / gate_rows, so gate_rows = 1 is a gate of its own for every element, gate_rows = rows one per channel, and
+ * between them one per group of consecutive rows. branch == NULL: out = residual (the first norm of a network); residual == NULL: 0. One of the two must be
+ * there. out may be NULL (not stored) or residual itself (same pitch); normed is there exactly when pre is not B200RL_NORM_NONE. pre sees the sum before it is
+ * rounded. dim <= B200RL_NORM_MAX_DIM. */
+int b200rl_norm_residual_forward(int type, int post, const float* post_weight, const float* post_bias, const void* branch, int ldb, const void* gate, int ldg,
+                                 int gate_rows, float scale, const void* residual, int ldr, void* out, int ldo, int pre, const float* pre_weight,
+                                 const float* pre_bias, void* normed, int ldn, int rows, int dim, float epsilon, b200rl_stream_t stream);
+
+/* The gradients of that pass. `out` is the sum that the forward pass stored, `branch`, `gate` and the parameters are its inputs (the statistics are
+ * computed again: nothing else is kept). d_out: gradient that reaches `out` along the residual stream (NULL: 0); d_normed: gradient of `normed` (NULL exactly
+ * when pre is B200RL_NORM_NONE).
+ *   d = d_out + (gradient of pre at out)^T d_normed;  d_residual = d;  d_gate = sum over the gate row's rows of scale u d;
+ *   d_branch = (gradient of post at branch)^T (scale gate d)
+ * d_residual, d_branch and d_gate (of `type`) and the four parameter gradients (fp32 [dim]) may each be NULL; accumulate != 0 adds onto the parameter
+ * gradients, 0 overwrites them. branch == NULL (no gradients but d_residual and those of pre) stands for a forward pass without one. d_residual may be d_out
+ * itself (same pitch). Sums over rows are taken in a fixed order. scratch: b200rl_norm_residual_backward_scratch_bytes, 16-byte aligned. */
+size_t b200rl_norm_residual_backward_scratch_bytes(int rows, int dim);
+int b200rl_norm_residual_backward(int type, int post, const float* post_weight, const float* post_bias, const void* branch, int ldb, const void* gate, int ldg,
+                                  int gate_rows, float scale, const void* out, int ldo, int pre, const float* pre_weight, const void* d_out, int lddo,
+                                  const void* d_normed, int lddn, void* d_branch, int lddb, void* d_residual, int lddr, void* d_gate, int lddg,
+                                  float* d_post_weight, float* d_post_bias, float* d_pre_weight, float* d_pre_bias, int accumulate, int rows, int dim,
+                                  float epsilon, void* scratch, size_t scratch_bytes, b200rl_stream_t stream);
+
+/* y = residual + (element kept ? x / P(kept) : 0), every type; residual may be NULL (0), y may be x or residual itself (same pitch). Element e = row * cols + col
+ * (whatever the pitches) is dropped when its 16 random bits are below floor(65536 p + 1/2): half e % 2 (low half first) of word e % 8 / 2 of the Philox block with
+ * the counter (b low, call low, call high, 2^31 + 2^16 (b >> 32) + stream_id), b = e / 8, keyed by seed; call = call_index + *call_counter (call_counter may be
+ * NULL). P(kept) is that of the rounded threshold; p = 1 drops everything. What is dropped is 0 whatever x holds there. The backward pass is the same call on the
+ * gradient with the same seed, stream_id and call. stream_id < 65536, rows * cols <= 2^50. Draws of other entry points use other counters. */
+int b200rl_dropout(int type, const void* x, int ldx, const void* residual, int ldr, void* y, int ldy, int rows, int cols, float p, unsigned long long seed,
+                   unsigned int stream_id, unsigned long long call_index, const unsigned long long* call_counter, b200rl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
