@@ -704,7 +704,7 @@ int b200rl_dense_residual_backward_input(int type, const void* W, int ldw, const
 /* d_W [output, input] (dense rows) = d_pre^T x and d_bias [output] = column sums of d_pre (either may be NULL), both fp32; accumulate != 0 adds onto
  * what they hold, 0 overwrites it. Every sum has a fixed order. The batch is summed in fp32 pieces of 512 rows, so that long batches lose nothing
  * to the tensor core's accumulator, which truncates. */
-size_t b200rl_dense_residual_backward_weights_workspace_bytes(const void* x, int ldx, const void* d_pre, int ldd, int batch, int input_dim, int output_dim);
+size_t b200rl_dense_residual_backward_weights_workspace_bytes(const void* x, int ldx, const void* d_pre, int ldd, const float* d_W, int batch, int input_dim, int output_dim);
 int b200rl_dense_residual_backward_weights(int type, const void* x, int ldx, const void* d_pre, int ldd, float* d_W, float* d_bias, int accumulate, int batch,
                                            int input_dim, int output_dim, void* workspace, size_t workspace_bytes, b200rl_stream_t stream);
 

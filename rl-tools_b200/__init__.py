@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libb200rl.so")
-SOURCES = ["dense.cu", "dense_tc.cu", "dense_skinny.cu", "mlp_fused.cu", "mlp_phase.cu", "grid_barrier.cu", "mlp_chain.cu", "mlp_grad.cu", "mlp_team.cu", "ppo_team.cu", "adam.cu", "rollout.cu", "rollout_tc.cu", "ppo.cu", "host_api.cu", "sac.cu", "normalize.cu", "rollout_env.cu", "l2f.cu", "dense_residual.cu", "norm_residual.cu", "dropout.cu"]
+SOURCES = ["dense.cu", "dense_tc.cu", "dense_skinny.cu", "mlp_fused.cu", "mlp_phase.cu", "grid_barrier.cu", "mlp_chain.cu", "mlp_grad.cu", "mlp_team.cu", "ppo_team.cu", "adam.cu", "rollout.cu", "rollout_tc.cu", "ppo.cu", "host_api.cu", "sac.cu", "normalize.cu", "rollout_env.cu", "l2f.cu", "dense_residual.cu", "product_tc.cu", "norm_residual.cu", "dropout.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared"]
 # per-source flags: the quadrotor dynamics keep the reference's association of every expression (bit-for-bit parity with its CPU step)
 SOURCE_FLAGS = {"l2f.cu": ["-fmad=false"]}
@@ -218,8 +218,8 @@ def lib():
         L.b200rl_pendulum_offpolicy_prologue.argtypes = [vp, vp, vp, vp, vp, u64, u64, vp, i, vp, vp, vp]
         L.b200rl_pendulum_offpolicy_epilogue.argtypes = [vp, vp, vp, vp, i, i, vp, vp, vp, vp, C.POINTER(ReplayLayout), vp, vp]
         L.b200rl_pendulum_rollout_device_rng.argtypes = [shape_p, vp, vp, vp, vp, vp, u64, u64, i, i, i, vp, vp, vp, vp, vp]
-        for name in ("forward", "backward_input", "backward_weights"):
-            getattr(L, f"b200rl_dense_residual_{name}_workspace_bytes").argtypes = [vp, i, vp, i, i, i, i]
+        for name, operands in (("forward", [vp, i, vp, i]), ("backward_input", [vp, i, vp, i]), ("backward_weights", [vp, i, vp, i, vp])):
+            getattr(L, f"b200rl_dense_residual_{name}_workspace_bytes").argtypes = operands + [i, i, i]
             getattr(L, f"b200rl_dense_residual_{name}_workspace_bytes").restype = sz
         L.b200rl_dense_residual_forward.argtypes = [i, vp, i, vp, vp, i, vp, i, f, vp, i, vp, i, i, i, i, i, vp, sz, vp]
         L.b200rl_dense_residual_backward_activation.argtypes = [i, vp, i, vp, i, f, vp, i, i, i, i, vp]

@@ -1,0 +1,725 @@
+// Products of 16-bit matrices on the tensor cores: operands by TMA into 128-byte-swizzled shared memory, tcgen05.mma with fp32 sums in tensor memory, the layer's epilogue on
+// the way out. C(m, n) = sum_k A(m, k) B(n, k); either operand may have k as the contiguous index of its matrix (the forward pass) or its row index (weights in the
+// input gradient, both operands in the weight gradient): TMA brings either form in, the operand descriptors say which it is, nothing is transposed.
+//
+// A CTA (or a pair of CTAs: CG = 2, one MMA over both SMs, each holding half of A and half of B) is persistent over output tiles of 128 CG x BN. Its warps:
+//   0  loads: stages of 64 k through a ring          1  issues the MMAs          2  holds the tensor memory
+//   4-11  epilogue: 32 rows x BN / 2 columns each, from one of two accumulators while the tensor core fills the other
+// Weight gradients and partial sums (EPI_SUM) are summed in pieces of PIECE k: the tensor core's accumulator truncates with every addition, which over a long batch adds up
+// (4,096 additions lose 1e-4); pieces of 32 additions are added in registers with rounding, while the next piece runs.
+#include "product.cuh"
+#include "tcgen05.cuh"
+#include <cuda.h>
+#include <atomic>
+
+namespace b200rl {
+
+namespace {
+constexpr int KB = 64;                                   // k of a stage: 128 bytes
+constexpr int PIECE = 512;                               // k in one accumulator of EPI_SUM
+constexpr int EPI_WARPS = 8, EPI_THREADS = EPI_WARPS * 32, THREADS = 128 + EPI_THREADS;
+constexpr uint32_t A_BYTES = 128 * 128;
+constexpr uint32_t STAGING = 8192;                       // per epilogue warp: two slabs of 32 x 32 of each output
+constexpr uint32_t SMEM_LIMIT = 232448;
+constexpr long long WAIT_LIMIT = 2000000000LL;           // cycles: about a second
+constexpr int SUM_COLUMNS = 16;                          // columns of a work item of the row sums: 32 bytes, a sector
+
+__host__ __device__ constexpr uint32_t stage_bytes(int CG, int BN){ return A_BYTES + (uint32_t)(BN / CG) * 128; }
+__host__ __device__ constexpr int stage_count(int CG, int BN){ return (int)((SMEM_LIMIT - 1024 - EPI_WARPS * STAGING - 512) / stage_bytes(CG, BN)) > 8 ? 8 : (int)((SMEM_LIMIT - 1024 - EPI_WARPS * STAGING - 512) / stage_bytes(CG, BN)); }
+__host__ __device__ constexpr uint32_t smem_bytes(int CG, int BN){ return 1024 + stage_count(CG, BN) * stage_bytes(CG, BN) + EPI_WARPS * STAGING + 512; }
+}
+
+__device__ int g_product_tc_error = 0;                   // set when a bounded wait ran out
+
+struct TcArgs {
+    int m, n, k;
+    int m_tiles, n_tiles, splits, split_blocks;          // split_blocks: k blocks of 64 in a split
+    uint32_t idesc;
+    const float* bias;
+    const void* add; long long ld_add;
+    void* pre; long long ld_pre;
+    void* out; long long ld_out;
+    float scale;
+    int act, accumulate;
+    int fast;                                            // 16-bit outputs by TMA, 16-byte loads of add and pre
+    const void* sum_source; long long ld_sum; float* sums; // row sums of A: [splits][m] (or the gradient itself: one split)
+    int sums_accumulate;
+};
+
+// ---- a tile's cooperating CTAs ------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank(){ uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t leader_address(const void* p){ uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(tc::smem_u32(p))); return r; }
+__device__ __forceinline__ void cluster_sync(){ asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void arrive_expect(uint64_t* bar, uint32_t bytes){ asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(tc::smem_u32(bar)), "r"(bytes) : "memory"); }
+template <int CG> __device__ __forceinline__ void arrive_at_leader(uint64_t* bar){
+    if constexpr(CG == 1) tc::mbar_arrive(bar);
+    else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(leader_address(bar)) : "memory");
+}
+// a box of a matrix into this CTA's shared memory; its bytes count at the leader's barrier
+template <int CG> __device__ __forceinline__ void load_box(void* smem, const CUtensorMap* map, int x, int y, uint64_t* bar){
+    if constexpr(CG == 1)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     :: "r"(tc::smem_u32(smem)), "l"(map), "r"(tc::smem_u32(bar)), "r"(x), "r"(y) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     :: "r"(tc::smem_u32(smem)), "l"(map), "r"(leader_address(bar)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void store_box_2d(const CUtensorMap* map, const void* smem, int x, int y){
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" :: "l"(map), "r"(tc::smem_u32(smem)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void store_box_3d(const CUtensorMap* map, const void* smem, int x, int y, int z){
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" :: "l"(map), "r"(tc::smem_u32(smem)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void add_box_3d(const CUtensorMap* map, const void* smem, int x, int y, int z){
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" :: "l"(map), "r"(tc::smem_u32(smem)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+template <int CG> __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate){
+    if constexpr(CG == 1) tc::mma_f16_ss(d, a, b, idesc, accumulate);
+    else asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
+                      :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
+}
+// arrives at the barrier (of both CTAs) when all MMAs issued so far have completed
+template <int CG> __device__ __forceinline__ void commit(uint64_t* bar){
+    if constexpr(CG == 1) tc::commit(bar);
+    else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" :: "r"(tc::smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+template <int CG> __device__ __forceinline__ void tensor_memory_alloc(uint32_t* slot, uint32_t columns){
+    if constexpr(CG == 1){ tc::tmem_alloc(slot, columns); tc::tmem_relinquish(); }
+    else{
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(tc::smem_u32(slot)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CG> __device__ __forceinline__ void tensor_memory_free(uint32_t address, uint32_t columns){
+    if constexpr(CG == 1) tc::tmem_dealloc(address, columns);
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(address), "r"(columns) : "memory");
+}
+// Descriptor of an operand whose rows are contiguous (k_rows), 128-byte swizzle: boxes of 64 rows of the operand x 64 k, [k][128 bytes], 8 k 1024 bytes apart (stride byte
+// offset), the next 64 rows of the operand 8192 bytes on (leading byte offset). 16 k further is 2048 bytes.
+__device__ __forceinline__ uint64_t make_desc_rows_sw128(uint32_t smem_addr){
+    return (uint64_t)((smem_addr >> 4) & 0x3FFF) | (uint64_t)(8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+struct TileIndex { int m, n, z; };
+// tiles in groups of eight rows of tiles, along the rows first: what runs at the same time shares operands in L2
+__device__ __forceinline__ TileIndex tile_index(const TcArgs& a, int t){
+    TileIndex i;
+    const int per_split = a.m_tiles * a.n_tiles;
+    i.z = t / per_split; t -= i.z * per_split;
+    const int group = t / (8 * a.n_tiles), first = group * 8, rows = min(8, a.m_tiles - first);
+    t -= group * 8 * a.n_tiles;
+    i.m = first + t % rows; i.n = t / rows;
+    return i;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float lo, float hi){ __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&v); }
+template <> __device__ __forceinline__ uint32_t pack<__half>(float lo, float hi){ __half2 v = __floats2half2_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&v); }
+template <typename T> __device__ __forceinline__ float2 unpack(uint32_t v);
+template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t v){ return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
+template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t v){ return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+
+// 32 consecutive elements of a row whose start is 16-byte aligned; elements from `end` on are 0
+template <typename T> __device__ __forceinline__ void load_slab_row(uint4 (&raw)[4], const T* row, int col, int end, bool there){
+#pragma unroll
+    for(int i = 0; i < 4; i++){
+        raw[i] = make_uint4(0, 0, 0, 0);
+        const int c = col + 8 * i;
+        if(!there || c >= end) continue;
+        if(c + 8 <= end) raw[i] = *reinterpret_cast<const uint4*>(row + c);
+        else{
+            union { uint4 v; T e[8]; } u;
+            u.v = raw[i];
+#pragma unroll
+            for(int j = 0; j < 8; j++) if(c + j < end) u.e[j] = row[c + j];
+            raw[i] = u.v;
+        }
+    }
+}
+// a row of a 32 x 32 slab of 16-bit elements, 64-byte swizzle
+template <typename T> __device__ __forceinline__ void store_slab_row(uint8_t* slab, int lane, const float (&v)[32]){
+#pragma unroll
+    for(int c = 0; c < 4; c++){
+        uint4 q = make_uint4(pack<T>(v[8 * c], v[8 * c + 1]), pack<T>(v[8 * c + 2], v[8 * c + 3]), pack<T>(v[8 * c + 4], v[8 * c + 5]), pack<T>(v[8 * c + 6], v[8 * c + 7]));
+        *reinterpret_cast<uint4*>(slab + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = q;
+    }
+}
+
+template <int ACT> __device__ __forceinline__ void activate(float (&v)[32]){
+#pragma unroll
+    for(int c = 0; c < 32; c++) v[c] = residual_activation<ACT>(v[c]);
+}
+template <int ACT> __device__ __forceinline__ void times_slope(float (&v)[32], const float (&p)[32]){
+#pragma unroll
+    for(int c = 0; c < 32; c++) v[c] *= residual_d_activation<ACT>(p[c]);
+}
+
+// One 32 x 32 slab whose operands or outputs have rows at odd addresses: transposed through shared memory, so that a lane has a column and every access of the warp goes
+// along a row.
+template <typename T, int EPI>
+__device__ __forceinline__ void finish_slab_by_rows(const TcArgs& a, float* buffer, const float (&v)[32], int row0, int col, int lane){
+#pragma unroll
+    for(int c = 0; c < 32; c++) buffer[lane * 33 + c] = v[c];
+    __syncwarp();
+    if(col < a.n){
+        const float bias = EPI == EPI_FORWARD && a.bias ? __ldg(a.bias + col) : 0.0f;
+        const int rows = min(32, a.m - row0);
+#pragma unroll 4
+        for(int r = 0; r < rows; r++){
+            const long long row = row0 + r;
+            float x = buffer[r * 33 + lane];
+            const float add = a.add ? to_float(static_cast<const T*>(a.add)[row * a.ld_add + col]) : 0.0f;
+            if constexpr(EPI == EPI_FORWARD){
+                x += bias;
+                if(a.pre) static_cast<T*>(a.pre)[row * a.ld_pre + col] = from_float<T>(x);
+                B200RL_DISPATCH_RESIDUAL_ACT(a.act, x = residual_activation<ACT>(x))
+                x = fmaf(a.scale, x, add);
+            }
+            else{
+                x += add;
+                if(a.act != B200RL_ACT_IDENTITY){
+                    const float p = to_float(static_cast<const T*>(a.pre)[row * a.ld_pre + col]);
+                    B200RL_DISPATCH_RESIDUAL_ACT(a.act, x *= residual_d_activation<ACT>(p))
+                }
+            }
+            static_cast<T*>(a.out)[row * a.ld_out + col] = from_float<T>(x);
+        }
+    }
+    __syncwarp();
+}
+
+template <typename T>
+__device__ __forceinline__ void sum_rows(const TcArgs& a, uint8_t* staging, int tid, int warp, int lane);
+
+template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI>
+__global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_pre,
+                                                                const __grid_constant__ TcArgs a){
+    constexpr int STAGES = stage_count(CG, BN);
+    constexpr uint32_t STAGE = stage_bytes(CG, BN);
+    constexpr int CW = BN / 2;                                          // columns of an epilogue warp
+    static_assert(CW % 32 == 0);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* staging = base + STAGES * STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + EPI_WARPS * STAGING);
+    uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + 2;
+    uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+    if(tid == 0){
+        for(int s = 0; s < STAGES; s++){ tc::mbar_init(full + s, 1); tc::mbar_init(empty + s, 1); }
+        for(int b = 0; b < 2; b++){ tc::mbar_init(acc_full + b, 1); tc::mbar_init(acc_empty + b, CG * EPI_WARPS); }
+        tc::fence_mbar_init();
+        *abort_flag = 0;
+    }
+    if(warp == 2) tensor_memory_alloc<CG>(slot, 2 * BN);
+    tc::fence_before_thread_sync();
+    __syncthreads();
+    if constexpr(CG == 2) cluster_sync();
+    tc::fence_after_thread_sync();
+    const uint32_t tmem = *slot;
+    const int tiles = a.m_tiles * a.n_tiles * a.splits, first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
+    const int k_blocks = (a.k + KB - 1) / KB;
+
+    if(warp < 4){
+        if constexpr(EPI == EPI_SUM) tc::setmaxnreg_dec<48>();
+        if(warp == 0 && lane == 0){
+            uint32_t it = 0;
+            bool ok = true;
+            for(int t = first_tile; t < tiles && ok; t += tile_step){
+                const TileIndex i = tile_index(a, t);
+                const int m0 = i.m * 128 * CG + (int)rank * 128, n0 = i.n * BN + (int)rank * (BN / CG);
+                const int kb_end = min(k_blocks, (i.z + 1) * a.split_blocks);
+                for(int kb = i.z * a.split_blocks; kb < kb_end; kb++, it++){
+                    const uint32_t s = it % STAGES, phase = (it / STAGES) & 1;
+                    if(!tc::mbar_wait_bounded(empty + s, phase ^ 1, WAIT_LIMIT) || *abort_flag){ ok = false; break; }
+                    uint8_t* stage = base + s * STAGE;
+                    if(rank == 0) arrive_expect(full + s, CG * STAGE);
+                    if constexpr(A_ROWS){
+                        load_box<CG>(stage, &map_a, m0, kb * KB, full + s);
+                        load_box<CG>(stage + 8192, &map_a, m0 + 64, kb * KB, full + s);
+                    }
+                    else load_box<CG>(stage, &map_a, kb * KB, m0, full + s);
+                    if constexpr(B_ROWS){
+#pragma unroll
+                        for(int j = 0; j < BN / CG / 64; j++) load_box<CG>(stage + A_BYTES + j * 8192, &map_b, n0 + 64 * j, kb * KB, full + s);
+                    }
+                    else load_box<CG>(stage + A_BYTES, &map_b, kb * KB, n0, full + s);
+                }
+            }
+            // no CTA leaves while its copies or its peer's signals are under way: the last use of every stage has been released
+            for(uint32_t s = 0; s < STAGES && s < it; s++){
+                const uint32_t last = (it - 1 - s) / STAGES * STAGES + s;         // the last step of this stage
+                if(!tc::mbar_wait_bounded(empty + s, (last / STAGES) & 1, WAIT_LIMIT)) ok = false;
+            }
+            if(!ok){ *abort_flag = 1; g_product_tc_error = 1; }
+        }
+        else if(warp == 1 && lane == 0 && rank == 0){
+            uint32_t it = 0, acc = 0;
+            bool ok = true;
+            for(int t = first_tile; t < tiles && ok; t += tile_step){
+                const int z = t / (a.m_tiles * a.n_tiles);
+                const int kb_end = min(k_blocks, (z + 1) * a.split_blocks);
+                for(int kb0 = z * a.split_blocks; kb0 < kb_end && ok; acc++){
+                    const int piece_end = EPI == EPI_SUM ? min(kb_end, kb0 + PIECE / KB) : kb_end;
+                    const uint32_t b = acc & 1, d = tmem + b * BN;
+                    if(!tc::mbar_wait_bounded(acc_empty + b, ((acc >> 1) & 1) ^ 1, WAIT_LIMIT)){ ok = false; break; }
+                    tc::fence_after_thread_sync();
+                    for(int kb = kb0; kb < piece_end; kb++, it++){
+                        const uint32_t s = it % STAGES;
+                        if(!tc::mbar_wait_bounded(full + s, (it / STAGES) & 1, WAIT_LIMIT) || *abort_flag){ ok = false; break; }
+                        tc::fence_after_thread_sync();
+                        const uint32_t stage = tc::smem_u32(base + s * STAGE);
+                        const uint64_t da = A_ROWS ? make_desc_rows_sw128(stage) : tc::make_desc_kmajor_sw128(stage);
+                        const uint64_t db = B_ROWS ? make_desc_rows_sw128(stage + A_BYTES) : tc::make_desc_kmajor_sw128(stage + A_BYTES);
+#pragma unroll
+                        for(int ks = 0; ks < KB / 16; ks++)
+                            mma<CG>(d, da + (uint64_t)(ks * (A_ROWS ? 128 : 2)), db + (uint64_t)(ks * (B_ROWS ? 128 : 2)), a.idesc, (kb > kb0 || ks) ? 1u : 0u);
+                        commit<CG>(empty + s);
+                    }
+                    if(!ok) break;
+                    commit<CG>(acc_full + b);
+                    kb0 = piece_end;
+                }
+            }
+            if(!ok){ *abort_flag = 1; g_product_tc_error = 1; }
+        }
+        __syncwarp();
+    }
+    else{
+        if constexpr(EPI == EPI_SUM) tc::setmaxnreg_inc<224>();
+        const int w = warp - 4, q = w & 3, half = w >> 2;                // tensor memory lanes 32 q .. +31, columns half CW .. +CW - 1
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        uint8_t* slabs = staging + w * STAGING;
+        if constexpr(EPI == EPI_SUM) if(a.sums) sum_rows<T>(a, staging, tid - 128, w, lane);
+        uint32_t acc = 0, stored = 0;
+        bool ok = true;
+        for(int t = first_tile; t < tiles && ok; t += tile_step){
+            const TileIndex i = tile_index(a, t);
+            const int row0 = i.m * 128 * CG + (int)rank * 128 + q * 32, col0 = i.n * BN + half * CW;
+            if constexpr(EPI == EPI_SUM){
+                const int kb_begin = i.z * a.split_blocks, kb_end = min(k_blocks, kb_begin + a.split_blocks);
+                const int pieces = (kb_end - kb_begin + PIECE / KB - 1) / (PIECE / KB);
+                float sum[CW / 32][32];
+#pragma unroll
+                for(int j = 0; j < CW / 32; j++)
+#pragma unroll
+                    for(int c = 0; c < 32; c++) sum[j][c] = 0.0f;
+                for(int p = 0; p < pieces; p++, acc++){
+                    const uint32_t b = acc & 1;
+                    if(!tc::mbar_wait_bounded(acc_full + b, (acc >> 1) & 1, WAIT_LIMIT)){ ok = false; break; }
+                    tc::fence_after_thread_sync();
+#pragma unroll
+                    for(int j = 0; j < CW / 32; j++){
+                        uint32_t r[32];
+                        tc::tmem_ld_32x32(tmem + lanes + b * BN + half * CW + j * 32, r);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for(int c = 0; c < 32; c++) sum[j][c] += __uint_as_float(r[c]);
+                    }
+                    tc::fence_before_thread_sync();
+                    __syncwarp();
+                    if(lane == 0) arrive_at_leader<CG>(acc_empty + b);
+                }
+                if(!ok) break;
+#pragma unroll
+                for(int j = 0; j < CW / 32; j++){
+                    uint8_t* slab = slabs + (stored & 1) * 4096;
+                    if(lane == 0) tc::bulk_wait_read<1>();
+                    __syncwarp();
+#pragma unroll
+                    for(int c = 0; c < 8; c++)
+                        *reinterpret_cast<float4*>(slab + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(sum[j][4 * c], sum[j][4 * c + 1], sum[j][4 * c + 2], sum[j][4 * c + 3]);
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if(lane == 0){
+                        if(row0 < a.m && col0 + j * 32 < a.n){
+                            if(a.accumulate) add_box_3d(&map_out, slab, col0 + j * 32, row0, i.z);
+                            else store_box_3d(&map_out, slab, col0 + j * 32, row0, i.z);
+                        }
+                        tc::bulk_commit();
+                    }
+                    stored++;
+                }
+            }
+            else{
+                const uint32_t b = acc & 1, phase = (acc >> 1) & 1;
+                acc++;
+                const long long row = row0 + lane;
+                const bool there = row < a.m && a.fast;
+                const T* add_row = a.add ? static_cast<const T*>(a.add) + row * a.ld_add : nullptr;
+                const T* pre_row = EPI == EPI_INPUT && a.act != B200RL_ACT_IDENTITY ? static_cast<const T*>(a.pre) + row * a.ld_pre : nullptr;
+                uint4 add_raw[4], pre_raw[4];
+                load_slab_row(add_raw, add_row, col0, a.n, there && add_row);
+                if constexpr(EPI == EPI_INPUT) load_slab_row(pre_raw, pre_row, col0, a.n, there && pre_row);
+                if(!tc::mbar_wait_bounded(acc_full + b, phase, WAIT_LIMIT)){ ok = false; break; }
+                tc::fence_after_thread_sync();
+#pragma unroll 1
+                for(int j = 0; j < CW / 32; j++){
+                    const int col = col0 + j * 32;
+                    uint32_t r[32];
+                    tc::tmem_ld_32x32(tmem + lanes + b * BN + half * CW + j * 32, r);
+                    tc::tmem_wait_ld();
+                    if(j == CW / 32 - 1){
+                        tc::fence_before_thread_sync();
+                        __syncwarp();
+                        if(lane == 0) arrive_at_leader<CG>(acc_empty + b);
+                    }
+                    if(row0 >= a.m || col >= a.n) continue;
+                    float v[32];
+#pragma unroll
+                    for(int c = 0; c < 32; c++) v[c] = __uint_as_float(r[c]);
+                    if(!a.fast){ finish_slab_by_rows<T, EPI>(a, reinterpret_cast<float*>(slabs), v, row0, col + lane, lane); continue; }
+                    float add[32];
+#pragma unroll
+                    for(int c = 0; c < 4; c++){
+                        const uint32_t u[4] = {add_raw[c].x, add_raw[c].y, add_raw[c].z, add_raw[c].w};
+#pragma unroll
+                        for(int e = 0; e < 4; e++){ const float2 f = unpack<T>(u[e]); add[8 * c + 2 * e] = f.x; add[8 * c + 2 * e + 1] = f.y; }
+                    }
+                    uint8_t *slab = slabs + (stored & 1) * 2048, *pre_slab = slabs + 4096 + (stored & 1) * 2048;
+                    if(lane == 0) tc::bulk_wait_read<1>();
+                    __syncwarp();
+                    if constexpr(EPI == EPI_FORWARD){
+                        if(a.bias)
+#pragma unroll
+                            for(int c = 0; c < 32; c++) v[c] += __ldg(a.bias + min(col + c, a.n - 1));
+                        if(a.pre) store_slab_row<T>(pre_slab, lane, v);
+                        if(j + 1 < CW / 32) load_slab_row(add_raw, add_row, col + 32, a.n, there && add_row);
+                        B200RL_DISPATCH_RESIDUAL_ACT(a.act, activate<ACT>(v))
+#pragma unroll
+                        for(int c = 0; c < 32; c++) v[c] = fmaf(a.scale, v[c], add[c]);
+                    }
+                    else{
+#pragma unroll
+                        for(int c = 0; c < 32; c++) v[c] += add[c];
+                        if(a.act != B200RL_ACT_IDENTITY){
+                            float p[32];
+#pragma unroll
+                            for(int c = 0; c < 4; c++){
+                                const uint32_t u[4] = {pre_raw[c].x, pre_raw[c].y, pre_raw[c].z, pre_raw[c].w};
+#pragma unroll
+                                for(int e = 0; e < 4; e++){ const float2 f = unpack<T>(u[e]); p[8 * c + 2 * e] = f.x; p[8 * c + 2 * e + 1] = f.y; }
+                            }
+                            if(j + 1 < CW / 32) load_slab_row(pre_raw, pre_row, col + 32, a.n, there && pre_row);
+                            B200RL_DISPATCH_RESIDUAL_ACT(a.act, times_slope<ACT>(v, p))
+                        }
+                        if(j + 1 < CW / 32) load_slab_row(add_raw, add_row, col + 32, a.n, there && add_row);
+                    }
+                    store_slab_row<T>(slab, lane, v);
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if(lane == 0){
+                        store_box_2d(&map_out, slab, col, row0);
+                        if constexpr(EPI == EPI_FORWARD) if(a.pre) store_box_2d(&map_pre, pre_slab, col, row0);
+                        tc::bulk_commit();
+                    }
+                    stored++;
+                }
+            }
+        }
+        if(!ok){ *abort_flag = 1; g_product_tc_error = 1; }
+        if(lane == 0) tc::bulk_wait_all<0>();
+        __syncwarp();
+    }
+    tc::fence_before_thread_sync();
+    __syncthreads();
+    if constexpr(CG == 2) cluster_sync();
+    tc::fence_after_thread_sync();
+    if(warp == 2) tensor_memory_free<CG>(tmem, 2 * BN);
+}
+
+// Row sums of A (the bias gradient) by the epilogue warps, before their first tile is due: item = 16 columns of A's matrix over one split of k, a thread a row in 256.
+template <typename T>
+__device__ __forceinline__ void sum_rows(const TcArgs& a, uint8_t* staging, int tid, int warp, int lane){
+    const int groups = (a.m + SUM_COLUMNS - 1) / SUM_COLUMNS, items = groups * a.splits;
+    float* shared = reinterpret_cast<float*>(staging);
+    for(int item = blockIdx.x; item < items; item += gridDim.x){
+        const int z = item / groups, c0 = (item - z * groups) * SUM_COLUMNS;
+        const long long begin = (long long)z * a.split_blocks * KB, end = min((long long)a.k, begin + (long long)a.split_blocks * KB);
+        float v[SUM_COLUMNS];
+#pragma unroll
+        for(int c = 0; c < SUM_COLUMNS; c++) v[c] = 0.0f;
+        for(long long k = begin + tid; k < end; k += EPI_THREADS){
+            const T* row = static_cast<const T*>(a.sum_source) + k * a.ld_sum + c0;        // 16-byte aligned
+            if(c0 + SUM_COLUMNS <= a.m){
+                float e[8];
+#pragma unroll
+                for(int h = 0; h < 2; h++){
+                    load_elements(row + 8 * h, e);
+#pragma unroll
+                    for(int c = 0; c < 8; c++) v[8 * h + c] += e[c];
+                }
+            }
+            else
+#pragma unroll
+                for(int c = 0; c < SUM_COLUMNS; c++) if(c0 + c < a.m) v[c] += to_float(row[c]);
+        }
+#pragma unroll
+        for(int c = 0; c < SUM_COLUMNS; c++)
+#pragma unroll
+            for(int o = 16; o > 0; o >>= 1) v[c] += __shfl_xor_sync(0xffffffffu, v[c], o);
+        if(lane == 0)
+#pragma unroll
+            for(int c = 0; c < SUM_COLUMNS; c++) shared[warp * SUM_COLUMNS + c] = v[c];
+        tc::named_barrier_sync(1, EPI_THREADS);
+        if(tid < SUM_COLUMNS && c0 + tid < a.m){
+            float total = 0.0f;
+#pragma unroll
+            for(int w = 0; w < EPI_WARPS; w++) total += shared[w * SUM_COLUMNS + tid];
+            float* out = a.sums + (long long)z * a.m + c0 + tid;
+            *out = a.sums_accumulate ? *out + total : total;
+        }
+        tc::named_barrier_sync(1, EPI_THREADS);
+    }
+}
+
+// ---- finishing partial sums -----------------------------------------------------------------------------------------------------------------------
+struct FinishArgs {
+    const float* partial; long long ld_partial, split_stride; int splits;
+    const float* row_sums;                               // [splits][m]
+    TcArgs a;
+    float* sums;
+};
+// out = epilogue(sum over the splits, in their order), a thread an element
+template <typename T, int EPI>
+__global__ void __launch_bounds__(256) finish_kernel(FinishArgs f){
+    const TcArgs& a = f.a;
+    const long long total = (long long)a.m * a.n;
+    for(long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll){
+        const long long row = i / a.n; const int col = (int)(i - row * a.n);
+        const float* p = f.partial + row * f.ld_partial + col;
+        float x = 0.0f;
+        for(int z = 0; z < f.splits; z++) x += p[z * f.split_stride];
+        if constexpr(EPI == EPI_SUM){
+            float* out = static_cast<float*>(a.out) + row * a.ld_out + col;
+            *out = a.accumulate ? *out + x : x;
+        }
+        else{
+            const float add = a.add ? to_float(static_cast<const T*>(a.add)[row * a.ld_add + col]) : 0.0f;
+            if constexpr(EPI == EPI_FORWARD){
+                if(a.bias) x += __ldg(a.bias + col);
+                if(a.pre) static_cast<T*>(a.pre)[row * a.ld_pre + col] = from_float<T>(x);
+                B200RL_DISPATCH_RESIDUAL_ACT(a.act, x = residual_activation<ACT>(x))
+                x = fmaf(a.scale, x, add);
+            }
+            else{
+                x += add;
+                if(a.act != B200RL_ACT_IDENTITY){
+                    const float q = to_float(static_cast<const T*>(a.pre)[row * a.ld_pre + col]);
+                    B200RL_DISPATCH_RESIDUAL_ACT(a.act, x *= residual_d_activation<ACT>(q))
+                }
+            }
+            static_cast<T*>(a.out)[row * a.ld_out + col] = from_float<T>(x);
+        }
+    }
+    if constexpr(EPI == EPI_SUM) if(f.row_sums)
+        for(int r = blockIdx.x * 256 + threadIdx.x; r < a.m; r += gridDim.x * 256){
+            float x = 0.0f;
+            for(int z = 0; z < f.splits; z++) x += f.row_sums[(long long)z * a.m + r];
+            f.sums[r] = a.sums_accumulate ? f.sums[r] + x : x;
+        }
+}
+
+// rows of 16-bit elements at any address -> rows that start on 16-byte boundaries, eight elements a thread
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* src, long long ld, uint16_t* dst, long long ld_dst, long long rows, int cols){
+    const int chunks = (int)(ld_dst / 8);
+    const long long total = rows * chunks;
+    for(long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll){
+        const long long r = i / chunks; const int c = (int)(i - r * chunks) * 8;
+        union { uint4 v; uint16_t e[8]; } u;
+#pragma unroll
+        for(int j = 0; j < 8; j++) u.e[j] = c + j < cols ? src[r * ld + c + j] : (uint16_t)0;
+        *reinterpret_cast<uint4*>(dst + r * ld_dst + c) = u.v;
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static int encode_tiled(EncodeTiled* out){
+    static std::atomic<EncodeTiled> cached{nullptr};
+    EncodeTiled f = cached.load(std::memory_order_relaxed);
+    if(!f){
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        B200RL_CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found));
+        if(found != cudaDriverEntryPointSuccess || !p) return B200RL_ERR_UNSUPPORTED;
+        f = reinterpret_cast<EncodeTiled>(p);
+        cached.store(f, std::memory_order_relaxed);
+    }
+    *out = f;
+    return B200RL_OK;
+}
+// rows x cols with rows ld elements apart, boxes of box_rows x box_cols; planes > 1 (or three): a third dimension plane_stride elements apart
+static int make_map(CUtensorMap* map, CUtensorMapDataType type, int element, const void* p, long long rows, long long cols, long long ld, int box_rows, int box_cols, CUtensorMapSwizzle swizzle,
+                    bool three = false, long long planes = 1, long long plane_stride = 0){
+    EncodeTiled encode;
+    int rc = encode_tiled(&encode);
+    if(rc) return rc;
+    // the pitch of a single row (or plane) is not used, but has to be a multiple of 16 bytes
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t pitch = rows > 1 ? (cuuint64_t)ld * element : ((cuuint64_t)cols * element + 15) / 16 * 16;
+    const cuuint64_t strides[2] = {pitch, planes > 1 ? (cuuint64_t)plane_stride * element : pitch * (cuuint64_t)rows};
+    const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, steps[3] = {1, 1, 1};
+    if(encode(map, type, three ? 3 : 2, const_cast<void*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return B200RL_ERR_UNSUPPORTED;
+    return B200RL_OK;
+}
+
+struct TcPlan {
+    int cg, bn, m_tiles, n_tiles, splits, split_blocks;
+    bool copy_a, copy_b, partial;
+    long long ld_copy_a, ld_copy_b, ld_partial;
+    size_t off_b, off_partial, off_sums, bytes;
+};
+static long long matrix_rows(const Operand& o, int r, int k){ return o.k_rows ? k : r; }
+static long long matrix_cols(const Operand& o, int r, int k){ return o.k_rows ? r : k; }
+static TcPlan plan_product(const Product& g, int epilogue){
+    TcPlan p{};
+    const int k_blocks = (g.k + KB - 1) / KB;
+    auto tiles_of = [&](int cg, int bn){ return (long long)((g.m + 128 * cg - 1) / (128 * cg)) * ((g.n + bn - 1) / bn); };
+    if(tiles_of(1, 128) >= 2 * NUM_SMS) { p.cg = 1; p.bn = 128; }
+    else { p.cg = 1; p.bn = 64; }
+    p.m_tiles = (g.m + 128 * p.cg - 1) / (128 * p.cg);
+    p.n_tiles = (g.n + p.bn - 1) / p.bn;
+    const long long tiles = (long long)p.m_tiles * p.n_tiles;
+    const int most = (k_blocks + PIECE / KB - 1) / (PIECE / KB);
+    p.splits = 1;
+    if(tiles * p.cg * 2 <= NUM_SMS){
+        p.splits = (int)(NUM_SMS / (tiles * p.cg));
+        if(p.splits > most) p.splits = most;
+    }
+    p.split_blocks = (k_blocks + p.splits - 1) / p.splits;
+    p.splits = (k_blocks + p.split_blocks - 1) / p.split_blocks;
+    // operands that TMA cannot address are copied
+    p.copy_a = !rows_aligned(g.a.p, g.a.ld, 2) && !(matrix_rows(g.a, g.m, g.k) <= 1 && reinterpret_cast<uintptr_t>(g.a.p) % 16 == 0);
+    p.copy_b = !rows_aligned(g.b.p, g.b.ld, 2) && !(matrix_rows(g.b, g.n, g.k) <= 1 && reinterpret_cast<uintptr_t>(g.b.p) % 16 == 0);
+    p.partial = p.splits > 1 || (epilogue == EPI_SUM && g.out && !rows_aligned(g.out, g.ld_out, 4));
+    p.ld_copy_a = (matrix_cols(g.a, g.m, g.k) + 7) / 8 * 8;
+    p.ld_copy_b = (matrix_cols(g.b, g.n, g.k) + 7) / 8 * 8;
+    p.ld_partial = (g.n + 31) / 32 * 32;
+    size_t at = 0;
+    auto take = [&](bool wanted, size_t bytes){ const size_t here = at; if(wanted) at += (bytes + 255) / 256 * 256; return here; };
+    take(p.copy_a, 2 * (size_t)p.ld_copy_a * matrix_rows(g.a, g.m, g.k));
+    p.off_b = take(p.copy_b, 2 * (size_t)p.ld_copy_b * matrix_rows(g.b, g.n, g.k));
+    p.off_partial = take(p.partial, sizeof(float) * (size_t)p.ld_partial * g.m * p.splits);
+    p.off_sums = take(p.splits > 1 && epilogue == EPI_SUM, sizeof(float) * (size_t)g.m * p.splits);
+    p.bytes = at;
+    return p;
+}
+size_t product_tc_workspace_bytes(const Product& g, int epilogue){ return plan_product(g, epilogue).bytes; }
+
+static int align_rows(const Operand& o, long long rows, long long cols, void* dst, long long ld_dst, cudaStream_t s){
+    const long long blocks = (rows * (ld_dst / 8) + 255) / 256;
+    align_rows_kernel<<<(unsigned)(blocks < NUM_SMS * 16 ? blocks : NUM_SMS * 16), 256, 0, s>>>(static_cast<const uint16_t*>(o.p), o.ld, static_cast<uint16_t*>(dst), ld_dst, rows, (int)cols);
+    B200RL_LAUNCH_CHECK("align_rows");
+    return B200RL_OK;
+}
+
+template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI>
+static int launch_tc(const CUtensorMap (&maps)[4], const TcArgs& a, cudaStream_t s){
+    auto* kernel = product_tc_kernel<CG, BN, A_ROWS, B_ROWS, T, EPI>;
+    static std::atomic<int> groups[MAX_DEVICES];           // tiles that run at the same time: 0 until the kernel is set up on the device
+    int dev = 0, sms = 0;
+    int rc = current_device(&dev);
+    if(rc || (rc = sm_count(&sms))) return rc;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = THREADS; cfg.dynamicSmemBytes = smem_bytes(CG, BN); cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = CG > 1 ? 1 : 0;
+    int most = groups[dev].load(std::memory_order_acquire);
+    if(most == 0){
+        B200RL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(CG, BN)));
+        most = sms;
+        if(CG > 1){
+            cfg.gridDim = sms / CG * CG;
+            B200RL_CUDA_TRY(cudaOccupancyMaxActiveClusters(&most, kernel, &cfg));
+            if(most < 1) return B200RL_ERR_UNSUPPORTED;
+        }
+        groups[dev].store(most, std::memory_order_release);
+    }
+    const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
+    cfg.gridDim = (unsigned)(CG * (tiles < most ? tiles : most));
+    B200RL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], a));
+    return B200RL_OK;
+}
+template <bool A_ROWS, bool B_ROWS, typename T, int EPI>
+static int launch_tile(const TcPlan& p, const CUtensorMap (&maps)[4], const TcArgs& a, cudaStream_t s){
+    if(p.cg == 1 && p.bn == 128) return launch_tc<1, 128, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
+    return launch_tc<1, 64, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
+}
+template <typename T, int EPI>
+static int launch_finish(const FinishArgs& f, cudaStream_t s){
+    const long long blocks = ((long long)f.a.m * f.a.n + 255) / 256;
+    finish_kernel<T, EPI><<<(unsigned)(blocks < NUM_SMS * 8 ? blocks : NUM_SMS * 8), 256, 0, s>>>(f);
+    B200RL_LAUNCH_CHECK("product finish");
+    return B200RL_OK;
+}
+
+template <typename T>
+static int product_tc_typed(const Product& g, int type, int epilogue, void* workspace, cudaStream_t s){
+    const TcPlan p = plan_product(g, epilogue);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    Operand A = g.a, B = g.b;
+    int rc;
+    if(p.copy_a){
+        if((rc = align_rows(A, matrix_rows(A, g.m, g.k), matrix_cols(A, g.m, g.k), ws, p.ld_copy_a, s))) return rc;
+        A.p = ws; A.ld = p.ld_copy_a;
+    }
+    if(p.copy_b){
+        if((rc = align_rows(B, matrix_rows(B, g.n, g.k), matrix_cols(B, g.n, g.k), ws + p.off_b, p.ld_copy_b, s))) return rc;
+        B.p = ws + p.off_b; B.ld = p.ld_copy_b;
+    }
+    float* partial = reinterpret_cast<float*>(ws + p.off_partial);
+    TcArgs a{};
+    a.m = g.m; a.n = g.n; a.k = g.k;
+    a.m_tiles = p.m_tiles; a.n_tiles = p.n_tiles; a.splits = p.splits; a.split_blocks = p.split_blocks;
+    const uint32_t format = type == B200RL_TYPE_BFLOAT16 ? 1u : 0u;
+    // fp32 sums, both operands of one type, their k_rows forms, N / 8, M / 16
+    a.idesc = 1u << 4 | format << 7 | format << 10 | (A.k_rows ? 1u << 15 : 0u) | (B.k_rows ? 1u << 16 : 0u) | (uint32_t)(p.bn / 8) << 17 | (uint32_t)(128 * p.cg / 16) << 24;
+    a.bias = g.bias; a.add = g.add; a.ld_add = g.ld_add; a.pre = g.pre; a.ld_pre = g.ld_pre; a.out = g.out; a.ld_out = g.ld_out;
+    a.scale = g.scale; a.act = g.act; a.accumulate = g.accumulate;
+    CUtensorMap maps[4] = {};
+    const CUtensorMapDataType dt = type == B200RL_TYPE_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if((rc = make_map(&maps[0], dt, 2, A.p, matrix_rows(A, g.m, g.k), matrix_cols(A, g.m, g.k), A.ld, A.k_rows ? 64 : 128, 64, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+    if((rc = make_map(&maps[1], dt, 2, B.p, matrix_rows(B, g.n, g.k), matrix_cols(B, g.n, g.k), B.ld, B.k_rows ? 64 : p.bn / p.cg, 64, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+    FinishArgs f{partial, p.ld_partial, p.ld_partial * (long long)g.m, p.splits, nullptr, a, g.row_sums};
+    if(epilogue == EPI_SUM || p.partial){
+        TcArgs b = a;
+        b.accumulate = p.partial ? 0 : g.accumulate;
+        float* out = p.partial ? partial : static_cast<float*>(g.out);
+        if((rc = make_map(&maps[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, out, g.m, g.n, p.partial ? p.ld_partial : g.ld_out, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, true, p.splits,
+                          f.split_stride))) return rc;
+        if(epilogue == EPI_SUM && g.row_sums){
+            b.sum_source = A.p; b.ld_sum = A.ld;
+            b.sums = p.splits > 1 ? reinterpret_cast<float*>(ws + p.off_sums) : g.row_sums;
+            b.sums_accumulate = p.splits > 1 ? 0 : g.accumulate;
+            f.row_sums = p.splits > 1 ? b.sums : nullptr;
+            f.a.sums_accumulate = g.accumulate;
+        }
+        if(A.k_rows && B.k_rows) rc = launch_tile<true, true, T, EPI_SUM>(p, maps, b, s);
+        else if(B.k_rows) rc = launch_tile<false, true, T, EPI_SUM>(p, maps, b, s);
+        else rc = launch_tile<false, false, T, EPI_SUM>(p, maps, b, s);
+        if(rc || !p.partial) return rc;
+        if(epilogue == EPI_SUM) return launch_finish<T, EPI_SUM>(f, s);
+        if(epilogue == EPI_INPUT) return launch_finish<T, EPI_INPUT>(f, s);
+        return launch_finish<T, EPI_FORWARD>(f, s);
+    }
+    a.fast = rows_aligned(g.out, g.ld_out, 2) && (!g.add || rows_aligned(g.add, g.ld_add, 2)) && (!g.pre || rows_aligned(g.pre, g.ld_pre, 2));
+    if(a.fast){
+        if((rc = make_map(&maps[2], dt, 2, g.out, g.m, g.n, g.ld_out, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
+        if(epilogue == EPI_FORWARD && g.pre && (rc = make_map(&maps[3], dt, 2, g.pre, g.m, g.n, g.ld_pre, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
+    }
+    if(epilogue == EPI_INPUT) return launch_tile<false, true, T, EPI_INPUT>(p, maps, a, s);
+    return launch_tile<false, false, T, EPI_FORWARD>(p, maps, a, s);
+}
+int product_tc(const Product& g, int type, int epilogue, void* workspace, cudaStream_t s){
+    B200RL_DISPATCH_16_BIT_TYPE(type, return (product_tc_typed<T>(g, type, epilogue, workspace, s)))
+}
+int product_tc_error_get(int* word){ B200RL_CUDA_TRY(cudaMemcpyFromSymbol(word, g_product_tc_error, sizeof(int))); return B200RL_OK; }
+int product_tc_error_clear(){ const int zero = 0; B200RL_CUDA_TRY(cudaMemcpyToSymbol(g_product_tc_error, &zero, sizeof(int))); return B200RL_OK; }
+
+}  // namespace b200rl

@@ -185,7 +185,7 @@ def dense_residual_backward(W, x, d_pre, d_W=None, d_bias=None, add=None, pre_in
     L = lib()
     # the weights first: d_in may overwrite what it reads, never x or d_pre
     if want_grads:
-        n = L.b200rl_dense_residual_backward_weights_workspace_bytes(px, ldx, pd, ldd, B, I, O)
+        n = L.b200rl_dense_residual_backward_weights_workspace_bytes(px, ldx, pd, ldd, d_W.data_ptr(), B, I, O)
         ws, pws = _workspace(n, d_pre.device)
         check(L.b200rl_dense_residual_backward_weights(o.type, px, ldx, pd, ldd, d_W.data_ptr(), pgb, len(given) > 0, B, I, O, pws, n, _stream()), call)
     if want_d_in:
