@@ -581,7 +581,8 @@ static TcPlan plan_product(const Product& g, int epilogue){
     TcPlan p{};
     const int k_blocks = (g.k + KB - 1) / KB;
     auto tiles_of = [&](int cg, int bn){ return (long long)((g.m + 128 * cg - 1) / (128 * cg)) * ((g.n + bn - 1) / bn); };
-    if(tiles_of(1, 128) >= 2 * NUM_SMS) { p.cg = 1; p.bn = 128; }
+    if(tiles_of(2, 256) >= NUM_SMS / 2 - 10) { p.cg = 2; p.bn = 256; }
+    else if(tiles_of(1, 128) >= NUM_SMS - 20) { p.cg = 1; p.bn = 128; }
     else { p.cg = 1; p.bn = 64; }
     p.m_tiles = (g.m + 128 * p.cg - 1) / (128 * p.cg);
     p.n_tiles = (g.n + p.bn - 1) / p.bn;
@@ -648,7 +649,8 @@ static int launch_tc(const CUtensorMap (&maps)[4], const TcArgs& a, cudaStream_t
 }
 template <bool A_ROWS, bool B_ROWS, typename T, int EPI>
 static int launch_tile(const TcPlan& p, const CUtensorMap (&maps)[4], const TcArgs& a, cudaStream_t s){
-    if(p.cg == 1 && p.bn == 128) return launch_tc<1, 128, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
+    if(p.cg == 2) return launch_tc<2, 256, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
+    if(p.bn == 128) return launch_tc<1, 128, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
     return launch_tc<1, 64, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
 }
 template <typename T, int EPI>
