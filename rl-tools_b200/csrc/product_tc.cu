@@ -3,7 +3,7 @@
 // input gradient, both operands in the weight gradient): TMA brings either form in, the operand descriptors say which it is, nothing is transposed.
 //
 // A CTA (or a pair of CTAs: CG = 2, one MMA over both SMs, each holding half of A and half of B) is persistent over output tiles of 128 CG x BN. Its warps:
-//   0  loads: stages of 64 k through a ring          1  issues the MMAs          2  holds the tensor memory
+//   0  loads: stages of 64 k through a ring          1  issues the MMAs          2, 3  row sums of A (the bias gradient), straight from its matrix, beside the products
 //   4-11  epilogue: 32 rows x BN / 2 columns each, from one of two accumulators while the tensor core fills the other
 // Weight gradients and partial sums (EPI_SUM) are summed in pieces of PIECE k: the tensor core's accumulator truncates with every addition, which over a long batch adds up
 // (4,096 additions lose 1e-4); pieces of 32 additions are added in registers with rounding, while the next piece runs.
@@ -19,10 +19,10 @@ constexpr int KB = 64;                                   // k of a stage: 128 by
 constexpr int PIECE = 512;                               // k in one accumulator of EPI_SUM
 constexpr int EPI_WARPS = 8, EPI_THREADS = EPI_WARPS * 32, THREADS = 128 + EPI_THREADS;
 constexpr uint32_t A_BYTES = 128 * 128;
-constexpr uint32_t STAGING = 8192;                       // per epilogue warp: two slabs of 32 x 32 of each output
+constexpr uint32_t STAGING = 8192;                       // per epilogue warp: two slabs of 32 rows x up to 128 bytes
 constexpr uint32_t SMEM_LIMIT = 232448;
 constexpr long long WAIT_LIMIT = 2000000000LL;           // cycles: about a second
-constexpr int SUM_COLUMNS = 16;                          // columns of a work item of the row sums: 32 bytes, a sector
+constexpr int SUM_COLUMNS = 16, SUM_THREADS = 64;        // columns of a work item of the row sums: 32 bytes, a sector
 
 __host__ __device__ constexpr uint32_t stage_bytes(int CG, int BN){ return A_BYTES + (uint32_t)(BN / CG) * 128; }
 __host__ __device__ constexpr int stage_count(int CG, int BN){ return (int)((SMEM_LIMIT - 1024 - EPI_WARPS * STAGING - 512) / stage_bytes(CG, BN)) > 8 ? 8 : (int)((SMEM_LIMIT - 1024 - EPI_WARPS * STAGING - 512) / stage_bytes(CG, BN)); }
@@ -64,6 +64,7 @@ template <int CG> __device__ __forceinline__ void load_box(void* smem, const CUt
         asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                      :: "r"(tc::smem_u32(smem)), "l"(map), "r"(leader_address(bar)), "r"(x), "r"(y) : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map){ asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory"); }
 __device__ __forceinline__ void store_box_2d(const CUtensorMap* map, const void* smem, int x, int y){
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" :: "l"(map), "r"(tc::smem_u32(smem)), "r"(x), "r"(y) : "memory");
 }
@@ -119,10 +120,10 @@ template <typename T> __device__ __forceinline__ float2 unpack(uint32_t v);
 template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t v){ return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t v){ return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
-// 32 consecutive elements of a row whose start is 16-byte aligned; elements from `end` on are 0
-template <typename T> __device__ __forceinline__ void load_slab_row(uint4 (&raw)[4], const T* row, int col, int end, bool there){
+// 8 N consecutive elements of a row whose start is 16-byte aligned; elements from `end` on are 0
+template <typename T, int N> __device__ __forceinline__ void load_slab_row(uint4 (&raw)[N], const T* row, int col, int end, bool there){
 #pragma unroll
-    for(int i = 0; i < 4; i++){
+    for(int i = 0; i < N; i++){
         raw[i] = make_uint4(0, 0, 0, 0);
         const int c = col + 8 * i;
         if(!there || c >= end) continue;
@@ -136,33 +137,47 @@ template <typename T> __device__ __forceinline__ void load_slab_row(uint4 (&raw)
         }
     }
 }
-// a row of a 32 x 32 slab of 16-bit elements, 64-byte swizzle
-template <typename T> __device__ __forceinline__ void store_slab_row(uint8_t* slab, int lane, const float (&v)[32]){
+// a row of a slab of 32 rows x W 16-bit elements, as the tensor maps of the outputs have it: rows of 64 bytes with the 64-byte swizzle or of 128 with the 128-byte one
+template <typename T, int W> __device__ __forceinline__ void store_slab_row(uint8_t* slab, int lane, const float (&v)[W]){
 #pragma unroll
-    for(int c = 0; c < 4; c++){
+    for(int c = 0; c < W / 8; c++){
         uint4 q = make_uint4(pack<T>(v[8 * c], v[8 * c + 1]), pack<T>(v[8 * c + 2], v[8 * c + 3]), pack<T>(v[8 * c + 4], v[8 * c + 5]), pack<T>(v[8 * c + 6], v[8 * c + 7]));
-        *reinterpret_cast<uint4*>(slab + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = q;
+        *reinterpret_cast<uint4*>(slab + lane * (2 * W) + ((c ^ (W == 64 ? lane & 7 : (lane >> 1) & 3)) << 4)) = q;
+    }
+}
+template <typename T, int N> __device__ __forceinline__ void unpack_chunk(float (&f)[8], const uint4 (&raw)[N], int i){
+    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+    for(int e = 0; e < 4; e++){ const float2 p = unpack<T>(u[e]); f[2 * e] = p.x; f[2 * e + 1] = p.y; }
+}
+template <int ACT, int W> __device__ __forceinline__ void activate(float (&v)[W]){
+#pragma unroll
+    for(int c = 0; c < W; c++) v[c] = residual_activation<ACT>(v[c]);
+}
+template <int ACT, typename T, int W> __device__ __forceinline__ void times_slope(float (&v)[W], const uint4 (&pre)[W / 8]){
+#pragma unroll
+    for(int i = 0; i < W / 8; i++){
+        float p[8];
+        unpack_chunk<T>(p, pre, i);
+#pragma unroll
+        for(int c = 0; c < 8; c++) v[8 * i + c] *= residual_d_activation<ACT>(p[c]);
     }
 }
 
-template <int ACT> __device__ __forceinline__ void activate(float (&v)[32]){
+template <int N> __device__ __forceinline__ void load_bias(float (&bias)[N], const TcArgs& a, int col){
 #pragma unroll
-    for(int c = 0; c < 32; c++) v[c] = residual_activation<ACT>(v[c]);
-}
-template <int ACT> __device__ __forceinline__ void times_slope(float (&v)[32], const float (&p)[32]){
-#pragma unroll
-    for(int c = 0; c < 32; c++) v[c] *= residual_d_activation<ACT>(p[c]);
+    for(int h = 0; h < N; h++) bias[h] = a.bias && col + 32 * h < a.n ? a.bias[col + 32 * h] : 0.0f;
 }
 
 // One 32 x 32 slab whose operands or outputs have rows at odd addresses: transposed through shared memory, so that a lane has a column and every access of the warp goes
 // along a row.
 template <typename T, int EPI>
-__device__ __forceinline__ void finish_slab_by_rows(const TcArgs& a, float* buffer, const float (&v)[32], int row0, int col, int lane){
+__device__ __forceinline__ void finish_slab_by_rows(const TcArgs& a, float* buffer, const float* v, int row0, int col, int lane){
 #pragma unroll
     for(int c = 0; c < 32; c++) buffer[lane * 33 + c] = v[c];
     __syncwarp();
     if(col < a.n){
-        const float bias = EPI == EPI_FORWARD && a.bias ? __ldg(a.bias + col) : 0.0f;
+        const float bias = EPI == EPI_FORWARD && a.bias ? a.bias[col] : 0.0f;
         const int rows = min(32, a.m - row0);
 #pragma unroll 4
         for(int r = 0; r < rows; r++){
@@ -189,7 +204,7 @@ __device__ __forceinline__ void finish_slab_by_rows(const TcArgs& a, float* buff
 }
 
 template <typename T>
-__device__ __forceinline__ void sum_rows(const TcArgs& a, uint8_t* staging, int tid, int warp, int lane);
+__device__ __forceinline__ void sum_rows(const TcArgs& a, float* shared, int tid, int warp, int lane);
 
 template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI>
 __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -197,8 +212,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                                                                 const __grid_constant__ TcArgs a){
     constexpr int STAGES = stage_count(CG, BN);
     constexpr uint32_t STAGE = stage_bytes(CG, BN);
-    constexpr int CW = BN / 2;                                          // columns of an epilogue warp
-    static_assert(CW % 32 == 0);
+    constexpr int CW = BN / 2, SW = CW < 64 ? CW : 64;                  // columns of an epilogue warp, of a slab of 16-bit outputs
+    static_assert(CW % SW == 0 && SW % 32 == 0);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* staging = base + STAGES * STAGE;
@@ -206,9 +221,11 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + 2;
     uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+    float* sum_buffer = reinterpret_cast<float*>(slot + 4);                  // [2][SUM_COLUMNS]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
     if(tid == 0){
+        prefetch_map(&map_a); prefetch_map(&map_b); prefetch_map(&map_out); prefetch_map(&map_pre);
         for(int s = 0; s < STAGES; s++){ tc::mbar_init(full + s, 1); tc::mbar_init(empty + s, 1); }
         for(int b = 0; b < 2; b++){ tc::mbar_init(acc_full + b, 1); tc::mbar_init(acc_empty + b, CG * EPI_WARPS); }
         tc::fence_mbar_init();
@@ -220,11 +237,12 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     if constexpr(CG == 2) cluster_sync();
     tc::fence_after_thread_sync();
     const uint32_t tmem = *slot;
+    after_predecessor();
     const int tiles = a.m_tiles * a.n_tiles * a.splits, first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
     const int k_blocks = (a.k + KB - 1) / KB;
 
     if(warp < 4){
-        if constexpr(EPI == EPI_SUM) tc::setmaxnreg_dec<48>();
+        tc::setmaxnreg_dec<72>();
         if(warp == 0 && lane == 0){
             uint32_t it = 0;
             bool ok = true;
@@ -286,14 +304,14 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             }
             if(!ok){ *abort_flag = 1; g_product_tc_error = 1; }
         }
+        else if(EPI == EPI_SUM && warp >= 2 && a.sums) sum_rows<T>(a, sum_buffer, tid - 64, warp - 2, lane);
         __syncwarp();
     }
     else{
-        if constexpr(EPI == EPI_SUM) tc::setmaxnreg_inc<224>();
+        tc::setmaxnreg_inc<216>();
         const int w = warp - 4, q = w & 3, half = w >> 2;                // tensor memory lanes 32 q .. +31, columns half CW .. +CW - 1
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         uint8_t* slabs = staging + w * STAGING;
-        if constexpr(EPI == EPI_SUM) if(a.sums) sum_rows<T>(a, staging, tid - 128, w, lane);
         uint32_t acc = 0, stored = 0;
         bool ok = true;
         for(int t = first_tile; t < tiles && ok; t += tile_step){
@@ -312,12 +330,15 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     if(!tc::mbar_wait_bounded(acc_full + b, (acc >> 1) & 1, WAIT_LIMIT)){ ok = false; break; }
                     tc::fence_after_thread_sync();
 #pragma unroll
-                    for(int j = 0; j < CW / 32; j++){
-                        uint32_t r[32];
-                        tc::tmem_ld_32x32(tmem + lanes + b * BN + half * CW + j * 32, r);
+                    for(int j = 0; j < CW / 32; j += SW / 32){
+                        uint32_t r[SW / 32][32];
+#pragma unroll
+                        for(int h = 0; h < SW / 32; h++) tc::tmem_ld_32x32(tmem + lanes + b * BN + half * CW + (j + h) * 32, r[h]);
                         tc::tmem_wait_ld();
 #pragma unroll
-                        for(int c = 0; c < 32; c++) sum[j][c] += __uint_as_float(r[c]);
+                        for(int h = 0; h < SW / 32; h++)
+#pragma unroll
+                            for(int c = 0; c < 32; c++) sum[j + h][c] += __uint_as_float(r[h][c]);
                     }
                     tc::fence_before_thread_sync();
                     __syncwarp();
@@ -351,69 +372,86 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 const bool there = row < a.m && a.fast;
                 const T* add_row = a.add ? static_cast<const T*>(a.add) + row * a.ld_add : nullptr;
                 const T* pre_row = EPI == EPI_INPUT && a.act != B200RL_ACT_IDENTITY ? static_cast<const T*>(a.pre) + row * a.ld_pre : nullptr;
-                uint4 add_raw[4], pre_raw[4];
+                uint4 add_raw[SW / 8], pre_raw[EPI == EPI_INPUT ? SW / 8 : 1];
+                float bias[SW / 32];                                     // of columns lane, lane + 32
                 load_slab_row(add_raw, add_row, col0, a.n, there && add_row);
                 if constexpr(EPI == EPI_INPUT) load_slab_row(pre_raw, pre_row, col0, a.n, there && pre_row);
+                else load_bias(bias, a, col0 + lane);
                 if(!tc::mbar_wait_bounded(acc_full + b, phase, WAIT_LIMIT)){ ok = false; break; }
                 tc::fence_after_thread_sync();
 #pragma unroll 1
-                for(int j = 0; j < CW / 32; j++){
-                    const int col = col0 + j * 32;
-                    uint32_t r[32];
-                    tc::tmem_ld_32x32(tmem + lanes + b * BN + half * CW + j * 32, r);
-                    tc::tmem_wait_ld();
-                    if(j == CW / 32 - 1){
+                for(int j = 0; j < CW / SW; j++){
+                    const int col = col0 + j * SW;
+                    float v[SW];
+                    {
+                        uint32_t r[SW / 32][32];
+#pragma unroll
+                        for(int h = 0; h < SW / 32; h++) tc::tmem_ld_32x32(tmem + lanes + b * BN + half * CW + j * SW + h * 32, r[h]);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for(int c = 0; c < SW; c++) v[c] = __uint_as_float(r[c / 32][c % 32]);
+                    }
+                    if(j == CW / SW - 1){
                         tc::fence_before_thread_sync();
                         __syncwarp();
                         if(lane == 0) arrive_at_leader<CG>(acc_empty + b);
                     }
                     if(row0 >= a.m || col >= a.n) continue;
-                    float v[32];
+                    if(!a.fast){
 #pragma unroll
-                    for(int c = 0; c < 32; c++) v[c] = __uint_as_float(r[c]);
-                    if(!a.fast){ finish_slab_by_rows<T, EPI>(a, reinterpret_cast<float*>(slabs), v, row0, col + lane, lane); continue; }
-                    float add[32];
-#pragma unroll
-                    for(int c = 0; c < 4; c++){
-                        const uint32_t u[4] = {add_raw[c].x, add_raw[c].y, add_raw[c].z, add_raw[c].w};
-#pragma unroll
-                        for(int e = 0; e < 4; e++){ const float2 f = unpack<T>(u[e]); add[8 * c + 2 * e] = f.x; add[8 * c + 2 * e + 1] = f.y; }
+                        for(int h = 0; h < SW / 32; h++) finish_slab_by_rows<T, EPI>(a, reinterpret_cast<float*>(slabs), v + 32 * h, row0, col + 32 * h + lane, lane);
+                        continue;
                     }
-                    uint8_t *slab = slabs + (stored & 1) * 2048, *pre_slab = slabs + 4096 + (stored & 1) * 2048;
-                    if(lane == 0) tc::bulk_wait_read<1>();
+                    // two slabs in turn; with pre-activations to keep, one for each output
+                    const bool two = EPI == EPI_FORWARD && a.pre;
+                    uint8_t *slab = slabs + (two ? 0 : (stored & 1) * 4096), *pre_slab = slabs + 4096;
+                    if(lane == 0){ if(two) tc::bulk_wait_read<0>(); else tc::bulk_wait_read<1>(); }
                     __syncwarp();
                     if constexpr(EPI == EPI_FORWARD){
-                        if(a.bias)
+                        if(a.bias){                                      // a lane needs every column's: handed round through the slab
+                            float* all = reinterpret_cast<float*>(slab);
 #pragma unroll
-                            for(int c = 0; c < 32; c++) v[c] += __ldg(a.bias + min(col + c, a.n - 1));
-                        if(a.pre) store_slab_row<T>(pre_slab, lane, v);
-                        if(j + 1 < CW / 32) load_slab_row(add_raw, add_row, col + 32, a.n, there && add_row);
+                            for(int h = 0; h < SW / 32; h++) all[h * 32 + lane] = bias[h];
+                            __syncwarp();
+#pragma unroll
+                            for(int c = 0; c < SW; c += 4){
+                                const float4 q = *reinterpret_cast<const float4*>(all + c);
+                                v[c] += q.x; v[c + 1] += q.y; v[c + 2] += q.z; v[c + 3] += q.w;
+                            }
+                            __syncwarp();
+                            if(j + 1 < CW / SW) load_bias(bias, a, col + SW + lane);
+                        }
+                        if(a.pre) store_slab_row<T, SW>(pre_slab, lane, v);
                         B200RL_DISPATCH_RESIDUAL_ACT(a.act, activate<ACT>(v))
 #pragma unroll
-                        for(int c = 0; c < 32; c++) v[c] = fmaf(a.scale, v[c], add[c]);
+                        for(int i = 0; i < SW / 8; i++){
+                            float add[8];
+                            unpack_chunk<T>(add, add_raw, i);
+#pragma unroll
+                            for(int c = 0; c < 8; c++) v[8 * i + c] = fmaf(a.scale, v[8 * i + c], add[c]);
+                        }
+                        if(j + 1 < CW / SW) load_slab_row(add_raw, add_row, col + SW, a.n, there && add_row);
                     }
                     else{
 #pragma unroll
-                        for(int c = 0; c < 32; c++) v[c] += add[c];
-                        if(a.act != B200RL_ACT_IDENTITY){
-                            float p[32];
+                        for(int i = 0; i < SW / 8; i++){
+                            float add[8];
+                            unpack_chunk<T>(add, add_raw, i);
 #pragma unroll
-                            for(int c = 0; c < 4; c++){
-                                const uint32_t u[4] = {pre_raw[c].x, pre_raw[c].y, pre_raw[c].z, pre_raw[c].w};
-#pragma unroll
-                                for(int e = 0; e < 4; e++){ const float2 f = unpack<T>(u[e]); p[8 * c + 2 * e] = f.x; p[8 * c + 2 * e + 1] = f.y; }
-                            }
-                            if(j + 1 < CW / 32) load_slab_row(pre_raw, pre_row, col + 32, a.n, there && pre_row);
-                            B200RL_DISPATCH_RESIDUAL_ACT(a.act, times_slope<ACT>(v, p))
+                            for(int c = 0; c < 8; c++) v[8 * i + c] += add[c];
                         }
-                        if(j + 1 < CW / 32) load_slab_row(add_raw, add_row, col + 32, a.n, there && add_row);
+                        if(j + 1 < CW / SW) load_slab_row(add_raw, add_row, col + SW, a.n, there && add_row);
+                        if(a.act != B200RL_ACT_IDENTITY){
+                            B200RL_DISPATCH_RESIDUAL_ACT(a.act, (times_slope<ACT, T, SW>(v, pre_raw)))
+                            if(j + 1 < CW / SW) load_slab_row(pre_raw, pre_row, col + SW, a.n, there && pre_row);
+                        }
                     }
-                    store_slab_row<T>(slab, lane, v);
+                    store_slab_row<T, SW>(slab, lane, v);
                     tc::fence_proxy_async_smem();
                     __syncwarp();
                     if(lane == 0){
                         store_box_2d(&map_out, slab, col, row0);
-                        if constexpr(EPI == EPI_FORWARD) if(a.pre) store_box_2d(&map_pre, pre_slab, col, row0);
+                        if(two) store_box_2d(&map_pre, pre_slab, col, row0);
                         tc::bulk_commit();
                     }
                     stored++;
@@ -431,32 +469,49 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     if(warp == 2) tensor_memory_free<CG>(tmem, 2 * BN);
 }
 
-// Row sums of A (the bias gradient) by the epilogue warps, before their first tile is due: item = 16 columns of A's matrix over one split of k, a thread a row in 256.
+// Row sums of A (the bias gradient) by two warps that run beside the products: item = 16 columns of A's matrix over one split of k, a thread a row in 64, four rows of
+// loads under way at a time.
 template <typename T>
-__device__ __forceinline__ void sum_rows(const TcArgs& a, uint8_t* staging, int tid, int warp, int lane){
+__device__ __forceinline__ void sum_rows(const TcArgs& a, float* shared, int tid, int warp, int lane){
     const int groups = (a.m + SUM_COLUMNS - 1) / SUM_COLUMNS, items = groups * a.splits;
-    float* shared = reinterpret_cast<float*>(staging);
     for(int item = blockIdx.x; item < items; item += gridDim.x){
         const int z = item / groups, c0 = (item - z * groups) * SUM_COLUMNS;
         const long long begin = (long long)z * a.split_blocks * KB, end = min((long long)a.k, begin + (long long)a.split_blocks * KB);
+        const T* column = static_cast<const T*>(a.sum_source) + c0;                         // rows 16-byte aligned
         float v[SUM_COLUMNS];
 #pragma unroll
         for(int c = 0; c < SUM_COLUMNS; c++) v[c] = 0.0f;
-        for(long long k = begin + tid; k < end; k += EPI_THREADS){
-            const T* row = static_cast<const T*>(a.sum_source) + k * a.ld_sum + c0;        // 16-byte aligned
-            if(c0 + SUM_COLUMNS <= a.m){
-                float e[8];
+        if(c0 + SUM_COLUMNS <= a.m){
+            long long k = begin + tid;
+            for(; k + 3 * SUM_THREADS < end; k += 4 * SUM_THREADS){
+                uint4 raw[4][2];
+#pragma unroll
+                for(int i = 0; i < 4; i++)
+#pragma unroll
+                    for(int h = 0; h < 2; h++) raw[i][h] = *reinterpret_cast<const uint4*>(column + (k + i * SUM_THREADS) * a.ld_sum + 8 * h);
+#pragma unroll
+                for(int i = 0; i < 4; i++)
+#pragma unroll
+                    for(int h = 0; h < 2; h++){
+                        float e[8];
+                        unpack_chunk<T>(e, raw[i], h);
+#pragma unroll
+                        for(int c = 0; c < 8; c++) v[8 * h + c] += e[c];
+                    }
+            }
+            for(; k < end; k += SUM_THREADS)
 #pragma unroll
                 for(int h = 0; h < 2; h++){
-                    load_elements(row + 8 * h, e);
+                    float e[8];
+                    load_elements(column + k * a.ld_sum + 8 * h, e);
 #pragma unroll
                     for(int c = 0; c < 8; c++) v[8 * h + c] += e[c];
                 }
-            }
-            else
-#pragma unroll
-                for(int c = 0; c < SUM_COLUMNS; c++) if(c0 + c < a.m) v[c] += to_float(row[c]);
         }
+        else
+            for(long long k = begin + tid; k < end; k += SUM_THREADS)
+#pragma unroll
+                for(int c = 0; c < SUM_COLUMNS; c++) if(c0 + c < a.m) v[c] += to_float(column[k * a.ld_sum + c]);
 #pragma unroll
         for(int c = 0; c < SUM_COLUMNS; c++)
 #pragma unroll
@@ -464,15 +519,13 @@ __device__ __forceinline__ void sum_rows(const TcArgs& a, uint8_t* staging, int 
         if(lane == 0)
 #pragma unroll
             for(int c = 0; c < SUM_COLUMNS; c++) shared[warp * SUM_COLUMNS + c] = v[c];
-        tc::named_barrier_sync(1, EPI_THREADS);
+        tc::named_barrier_sync(1, SUM_THREADS);
         if(tid < SUM_COLUMNS && c0 + tid < a.m){
-            float total = 0.0f;
-#pragma unroll
-            for(int w = 0; w < EPI_WARPS; w++) total += shared[w * SUM_COLUMNS + tid];
+            const float total = shared[tid] + shared[SUM_COLUMNS + tid];
             float* out = a.sums + (long long)z * a.m + c0 + tid;
             *out = a.sums_accumulate ? *out + total : total;
         }
-        tc::named_barrier_sync(1, EPI_THREADS);
+        tc::named_barrier_sync(1, SUM_THREADS);
     }
 }
 
@@ -486,6 +539,7 @@ struct FinishArgs {
 // out = epilogue(sum over the splits, in their order), a thread an element
 template <typename T, int EPI>
 __global__ void __launch_bounds__(256) finish_kernel(FinishArgs f){
+    after_predecessor();
     const TcArgs& a = f.a;
     const long long total = (long long)a.m * a.n;
     for(long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll){
@@ -500,7 +554,7 @@ __global__ void __launch_bounds__(256) finish_kernel(FinishArgs f){
         else{
             const float add = a.add ? to_float(static_cast<const T*>(a.add)[row * a.ld_add + col]) : 0.0f;
             if constexpr(EPI == EPI_FORWARD){
-                if(a.bias) x += __ldg(a.bias + col);
+                if(a.bias) x += a.bias[col];
                 if(a.pre) static_cast<T*>(a.pre)[row * a.ld_pre + col] = from_float<T>(x);
                 B200RL_DISPATCH_RESIDUAL_ACT(a.act, x = residual_activation<ACT>(x))
                 x = fmaf(a.scale, x, add);
@@ -525,6 +579,7 @@ __global__ void __launch_bounds__(256) finish_kernel(FinishArgs f){
 
 // rows of 16-bit elements at any address -> rows that start on 16-byte boundaries, eight elements a thread
 __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* src, long long ld, uint16_t* dst, long long ld_dst, long long rows, int cols){
+    after_predecessor();
     const int chunks = (int)(ld_dst / 8);
     const long long total = rows * chunks;
     for(long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll){
@@ -615,8 +670,8 @@ size_t product_tc_workspace_bytes(const Product& g, int epilogue){ return plan_p
 
 static int align_rows(const Operand& o, long long rows, long long cols, void* dst, long long ld_dst, cudaStream_t s){
     const long long blocks = (rows * (ld_dst / 8) + 255) / 256;
-    align_rows_kernel<<<(unsigned)(blocks < NUM_SMS * 16 ? blocks : NUM_SMS * 16), 256, 0, s>>>(static_cast<const uint16_t*>(o.p), o.ld, static_cast<uint16_t*>(dst), ld_dst, rows, (int)cols);
-    B200RL_LAUNCH_CHECK("align_rows");
+    B200RL_CUDA_TRY(launch_after(align_rows_kernel, dim3((unsigned)(blocks < NUM_SMS * 16 ? blocks : NUM_SMS * 16)), dim3(256), 0, s, static_cast<const uint16_t*>(o.p), o.ld,
+                                 static_cast<uint16_t*>(dst), ld_dst, rows, (int)cols));
     return B200RL_OK;
 }
 
@@ -628,9 +683,10 @@ static int launch_tc(const CUtensorMap (&maps)[4], const TcArgs& a, cudaStream_t
     int rc = current_device(&dev);
     if(rc || (rc = sm_count(&sms))) return rc;
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.blockDim = THREADS; cfg.dynamicSmemBytes = smem_bytes(CG, BN); cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = CG > 1 ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.blockDim = THREADS; cfg.dynamicSmemBytes = smem_bytes(CG, BN); cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = 1;
     int most = groups[dev].load(std::memory_order_acquire);
     if(most == 0){
         B200RL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(CG, BN)));
@@ -644,6 +700,7 @@ static int launch_tc(const CUtensorMap (&maps)[4], const TcArgs& a, cudaStream_t
     }
     const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
     cfg.gridDim = (unsigned)(CG * (tiles < most ? tiles : most));
+    cfg.numAttrs = 2;
     B200RL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], a));
     return B200RL_OK;
 }
@@ -656,8 +713,7 @@ static int launch_tile(const TcPlan& p, const CUtensorMap (&maps)[4], const TcAr
 template <typename T, int EPI>
 static int launch_finish(const FinishArgs& f, cudaStream_t s){
     const long long blocks = ((long long)f.a.m * f.a.n + 255) / 256;
-    finish_kernel<T, EPI><<<(unsigned)(blocks < NUM_SMS * 8 ? blocks : NUM_SMS * 8), 256, 0, s>>>(f);
-    B200RL_LAUNCH_CHECK("product finish");
+    B200RL_CUDA_TRY(launch_after(finish_kernel<T, EPI>, dim3((unsigned)(blocks < NUM_SMS * 8 ? blocks : NUM_SMS * 8)), dim3(256), 0, s, f));
     return B200RL_OK;
 }
 
@@ -712,8 +768,10 @@ static int product_tc_typed(const Product& g, int type, int epilogue, void* work
     }
     a.fast = rows_aligned(g.out, g.ld_out, 2) && (!g.add || rows_aligned(g.add, g.ld_add, 2)) && (!g.pre || rows_aligned(g.pre, g.ld_pre, 2));
     if(a.fast){
-        if((rc = make_map(&maps[2], dt, 2, g.out, g.m, g.n, g.ld_out, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
-        if(epilogue == EPI_FORWARD && g.pre && (rc = make_map(&maps[3], dt, 2, g.pre, g.m, g.n, g.ld_pre, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
+        const int width = p.bn / 2 < 64 ? p.bn / 2 : 64;                 // of a slab
+        const CUtensorMapSwizzle swizzle = width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+        if((rc = make_map(&maps[2], dt, 2, g.out, g.m, g.n, g.ld_out, 32, width, swizzle))) return rc;
+        if(epilogue == EPI_FORWARD && g.pre && (rc = make_map(&maps[3], dt, 2, g.pre, g.m, g.n, g.ld_pre, 32, width, swizzle))) return rc;
     }
     if(epilogue == EPI_INPUT) return launch_tile<false, true, T, EPI_INPUT>(p, maps, a, s);
     return launch_tile<false, false, T, EPI_FORWARD>(p, maps, a, s);
