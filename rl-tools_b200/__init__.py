@@ -12,6 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libb200rl.so")
+TENSORS_PATH = os.path.join(HERE, "_tensors.so")
 SOURCES = ["dense.cu", "dense_tc.cu", "dense_skinny.cu", "mlp_fused.cu", "mlp_phase.cu", "grid_barrier.cu", "mlp_chain.cu", "mlp_grad.cu", "mlp_team.cu", "ppo_team.cu", "adam.cu", "rollout.cu", "rollout_tc.cu", "ppo.cu", "host_api.cu", "sac.cu", "normalize.cu", "rollout_env.cu", "l2f.cu", "dense_residual.cu", "product_tc.cu", "norm_residual.cu", "dropout.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared"]
 # per-source flags: the quadrotor dynamics keep the reference's association of every expression (bit-for-bit parity with its CPU step)
@@ -50,6 +51,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Compile every CUDA source into libb200rl.so for sm_100a (nvcc cross-compiles without a GPU)."""
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh")] + [os.path.join(ROOT, "include", "b200rl.h"), os.path.abspath(__file__)]
+    build_tensors(force)
     if not force and os.path.exists(LIB_PATH) and all(os.path.getmtime(LIB_PATH) >= os.path.getmtime(d) for d in deps):
         return LIB_PATH
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -80,6 +82,26 @@ def build(force: bool = False, verbose: bool = False) -> str:
         raise B200RLError("nvcc link failed:\n" + res.stdout + res.stderr)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
+
+
+def build_tensors(force: bool = False) -> str:
+    """Compile the calls of the residual operators on torch tensors (host code against torch's headers; it finds the library's entry points at run time)."""
+    src, header = os.path.join(CSRC, "tensors.cpp"), os.path.join(ROOT, "include", "b200rl.h")
+    if not force and os.path.exists(TENSORS_PATH) and all(os.path.getmtime(TENSORS_PATH) >= os.path.getmtime(d) for d in (src, header)):
+        return TENSORS_PATH
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    cuda = os.path.dirname(os.path.dirname(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")))
+    tmp = TENSORS_PATH + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    cmd += ["-isystem" + d for d in include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include")]]
+    cmd += [src, "-o", tmp, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise B200RLError("g++ failed on " + src + ":\n" + res.stdout + res.stderr)
+    os.replace(tmp, TENSORS_PATH)
+    return TENSORS_PATH
 
 
 class MlpShape(C.Structure):
