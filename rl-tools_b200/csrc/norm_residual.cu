@@ -4,6 +4,7 @@
 // d_residual and d_branch, each once. A row is held in the registers of 32, 128 or 512 threads as fp32, so the two passes of a variance (mean, then squared deviations)
 // cost no second read. The statistics are not stored for the backward pass: it holds the rows in registers anyway and computes them again.
 #include "residual.cuh"
+#include <atomic>
 #include <type_traits>
 
 namespace b200rl {
@@ -44,13 +45,14 @@ struct NormBackward {
 
 // Sums of N values over the threads of a row (one warp, or the whole CTA); every thread gets them. `buffer` is used in turns, so one barrier per call is enough.
 template <int TPR, int N>
-__device__ __forceinline__ void row_sums(float (&v)[N], float (*buffer)[N][TPR / 32], int& turn){
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*buffer)[4][TPR / 32], int& turn){
+    static_assert(N <= 4);
 #pragma unroll
-    for(int i = 0; i < N; i++)
+    for(int o = 16; o > 0; o >>= 1)
 #pragma unroll
-        for(int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        for(int i = 0; i < N; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     if constexpr(TPR > 32){
-        float (&shared)[N][TPR / 32] = buffer[turn];
+        float (&shared)[4][TPR / 32] = buffer[turn];
         turn ^= 1;
         const int warp = threadIdx.x >> 5;
         if((threadIdx.x & 31) == 0)
@@ -59,30 +61,68 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*buffer)[N][TPR /
         __syncthreads();
 #pragma unroll
         for(int i = 0; i < N; i++){
+            float4 part[TPR / 128];
+#pragma unroll
+            for(int w = 0; w < TPR / 128; w++) part[w] = *reinterpret_cast<const float4*>(&shared[i][4 * w]);
             v[i] = 0.0f;
 #pragma unroll
-            for(int w = 0; w < TPR / 32; w++) v[i] += shared[i][w];
+            for(int w = 0; w < TPR / 128; w++) v[i] += (part[w].x + part[w].y) + (part[w].z + part[w].w);
         }
     }
 }
+// The row's first element, which lies in v[0] of its first thread (N rows at once). A call of row_sums has to follow before the next one.
+template <int TPR, int N>
+__device__ __forceinline__ void row_first(float (&v)[N]){
+    if constexpr(TPR == 32){
+#pragma unroll
+        for(int i = 0; i < N; i++) v[i] = __shfl_sync(0xffffffffu, v[i], 0);
+    }
+    else{
+        __shared__ float first[N];
+        if(threadIdx.x == 0)
+#pragma unroll
+            for(int i = 0; i < N; i++) first[i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for(int i = 0; i < N; i++) v[i] = first[i];
+    }
+}
 
-// The row's elements of one thread: vectors of VEC, TPR VEC apart. What lies behind the row's end reads as `fill`.
+// The row's elements of one thread: vectors of VEC, TPR VEC apart. What lies behind the row's end reads as 0 (parameters: `fill`).
 template <typename T, int VEC, int TPR, int E>
 struct Row {
+    struct Raw { T e[E]; };
     int lane, dim;
     __device__ __forceinline__ int column(int i) const { return (i * TPR + lane) * VEC; }
-    __device__ __forceinline__ void load(const T* row, float (&v)[E]) const {
+    __device__ __forceinline__ bool inside(int e) const { return column(e / VEC) < dim; }
+    __device__ __forceinline__ void fetch(const void* base, long long at, Raw& raw) const {
+        const T* row = static_cast<const T*>(base) + at;
 #pragma unroll
         for(int i = 0; i < E / VEC; i++){
-            float e[VEC];
-#pragma unroll
-            for(int j = 0; j < VEC; j++) e[j] = 0.0f;
-            if(column(i) < dim) load_elements(row + column(i), e);
-#pragma unroll
-            for(int j = 0; j < VEC; j++) v[i * VEC + j] = e[j];
+            if constexpr(VEC > 1){
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if(column(i) < dim) v = *reinterpret_cast<const uint4*>(row + column(i));
+                *reinterpret_cast<uint4*>(&raw.e[i * VEC]) = v;
+            }
+            else raw.e[i] = column(i) < dim ? row[column(i)] : from_float<T>(0.0f);
         }
     }
-    __device__ __forceinline__ void store(T* row, const float (&v)[E]) const {
+    __device__ __forceinline__ void pairs(const Raw& raw, float2 (&v)[E / 2]) const {
+#pragma unroll
+        for(int i = 0; i < E / 2; i++) v[i] = make_float2(to_float(raw.e[2 * i]), to_float(raw.e[2 * i + 1]));
+    }
+    __device__ __forceinline__ void clear_outside(float2 (&v)[E / 2]) const {
+#pragma unroll
+        for(int i = 0; i < E / 2; i++){ if(!inside(2 * i)) v[i].x = 0.0f; if(!inside(2 * i + 1)) v[i].y = 0.0f; }
+    }
+    __device__ __forceinline__ void store(void* base, long long at, const float2 (&v)[E / 2]) const {
+        float f[E];
+#pragma unroll
+        for(int i = 0; i < E / 2; i++){ f[2 * i] = v[i].x; f[2 * i + 1] = v[i].y; }
+        store(base, at, f);
+    }
+    __device__ __forceinline__ void store(void* base, long long at, const float (&v)[E]) const {
+        T* row = static_cast<T*>(base) + at;
 #pragma unroll
         for(int i = 0; i < E / VEC; i++){
             float e[VEC];
@@ -91,269 +131,463 @@ struct Row {
             if(column(i) < dim) store_elements(row + column(i), e);
         }
     }
-    // fp32 parameters (NULL: `fill`)
     __device__ __forceinline__ void parameters(const float* p, float fill, float (&v)[E]) const {
+        if(VEC > 1 && reinterpret_cast<uintptr_t>(p) % 16 == 0){
 #pragma unroll
-        for(int i = 0; i < E / VEC; i++)
+            for(int e = 0; e < E; e += 4){
+                float4 q = make_float4(fill, fill, fill, fill);
+                if(p && inside(e)) q = __ldg(reinterpret_cast<const float4*>(p + column(e / VEC) + e % VEC));
+                v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
+            }
+        }
+        else
 #pragma unroll
-            for(int j = 0; j < VEC; j++) v[i * VEC + j] = p && column(i) < dim ? __ldg(p + column(i) + j) : fill;
+            for(int e = 0; e < E; e++) v[e] = p && inside(e) ? __ldg(p + column(e / VEC) + e % VEC) : fill;
     }
-    __device__ __forceinline__ bool inside(int e) const { return column(e / VEC) < dim; }
 };
 
-// The row's first element, which lies in v[0] of its first thread. A call of row_sums has to follow before the next one.
-template <int TPR>
-__device__ __forceinline__ float row_first(float v){
-    if constexpr(TPR == 32) return __shfl_sync(0xffffffffu, v, 0);
-    else{
-        __shared__ float first;
-        if(threadIdx.x == 0) first = v;
-        __syncthreads();
-        return first;
-    }
+// Pairs of fp32 values: one instruction for both.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c){
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)), "l"(reinterpret_cast<const unsigned long long&>(c)));
+    return d;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b){
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b){
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v){ return make_float2(v, v); }
+__device__ __forceinline__ float across(float2 v){ return v.x + v.y; }
 
 // v <- (v - mean) rstd in place (0 behind the row's end); returns rstd. The mean is summed about the row's first element: a constant row has variance 0 whatever its value,
 // and the error of the mean goes by the row's spread.
-template <typename R, int TPR, int E>
-__device__ __forceinline__ float normalise(const R& row, int kind, float (&v)[E], float epsilon, float (*buffer)[1][TPR / 32], int& turn){
+template <int TPR, typename R, int P>
+__device__ __forceinline__ void normalise(const R& row, int kind, float2 (&v)[P], float epsilon, float (*buffer)[4][TPR / 32], int& turn){
     const float inv = 1.0f / (float)row.dim;
     if(kind == B200RL_NORM_LAYER){
-        const float first = row_first<TPR>(v[0]);
-        float s[1] = {0.0f};
+        float first[1] = {v[0].x}, s[1] = {0.0f};
+        row_first<TPR>(first);
 #pragma unroll
-        for(int e = 0; e < E; e++){ v[e] = row.inside(e) ? v[e] - first : 0.0f; s[0] += v[e]; }
+        for(int i = 0; i < P; i++) v[i] = add2(v[i], both(-first[0]));
+        row.clear_outside(v);
+#pragma unroll
+        for(int i = 0; i < P; i++) s[0] += across(v[i]);
         row_sums<TPR>(s, buffer, turn);
         const float mean = s[0] * inv;
 #pragma unroll
-        for(int e = 0; e < E; e++) v[e] = row.inside(e) ? v[e] - mean : 0.0f;
+        for(int i = 0; i < P; i++) v[i] = add2(v[i], both(-mean));
+        row.clear_outside(v);
     }
-    float s[1] = {0.0f};
+    float2 squares = both(0.0f);
 #pragma unroll
-    for(int e = 0; e < E; e++) s[0] = fmaf(v[e], v[e], s[0]);
+    for(int i = 0; i < P; i++) squares = fma2(v[i], v[i], squares);
+    float s[1] = {across(squares)};
     row_sums<TPR>(s, buffer, turn);
     const float rstd = 1.0f / sqrtf(s[0] * inv + epsilon);
 #pragma unroll
-    for(int e = 0; e < E; e++) v[e] *= rstd;
-    return rstd;
+    for(int i = 0; i < P; i++) v[i] = mul2(v[i], both(rstd));
 }
 
+// A CTA (or a warp, for short rows) takes every so many-th row. What a thread keeps over its rows, its columns' parameters, lies in shared memory at places of its own; the next
+// row's loads are under way while a row is summed.
 template <typename T, int VEC, int TPR, int E>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_forward_kernel(NormForward a){
-    constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
-    __shared__ float buffer[2][1][TPR / 32];
+    constexpr int ROWS = TPR < 128 ? 128 / TPR : 1, P = E / 2;
+    using R = Row<T, VEC, TPR, E>;
+    extern __shared__ __align__(16) float4 kept_memory[];                // [parameters that are there][ROWS][E / 4][TPR]
+    __shared__ __align__(16) float buffer[2][4][TPR / 32];
+    after_predecessor();
     int turn = 0;
-    const Row<T, VEC, TPR, E> R{(int)(threadIdx.x % TPR), a.dim};
-    for(long long r = (long long)blockIdx.x * ROWS + threadIdx.x / TPR; r < a.rows; r += (long long)gridDim.x * ROWS){
-        float o[E];
-        if(a.residual) R.load(static_cast<const T*>(a.residual) + r * a.ldr, o);
-        else
+    const R row{(int)(threadIdx.x % TPR), a.dim};
+    const float* const parameters[4] = {a.post_weight, a.post_bias, a.pre_weight, a.pre_bias};
+    int place[4], n = 0;
 #pragma unroll
-            for(int e = 0; e < E; e++) o[e] = 0.0f;
-        if(a.branch){
-            float u[E], p[E];
-            R.load(static_cast<const T*>(a.branch) + r * a.ldb, u);
-            if(a.post != B200RL_NORM_NONE){
-                normalise<Row<T, VEC, TPR, E>, TPR>(R, a.post, u, a.epsilon, buffer, turn);
-                if(a.post_weight){
-                    R.parameters(a.post_weight, 1.0f, p);
+    for(int k = 0; k < 4; k++) if(parameters[k]) place[k] = n++; else place[k] = -1;
+    auto kept = [&](int k, int i) -> float4& { return kept_memory[((place[k] * ROWS + threadIdx.x / TPR) * (E / 4) + i) * TPR + threadIdx.x % TPR]; };
 #pragma unroll
-                    for(int e = 0; e < E; e++) u[e] *= p[e];
-                }
-                if(a.post_bias){
-                    R.parameters(a.post_bias, 0.0f, p);
-#pragma unroll
-                    for(int e = 0; e < E; e++) u[e] += p[e];
-                }
-            }
-            if(a.gate){
-                R.load(static_cast<const T*>(a.gate) + r / a.gate_rows * a.ldg, p);
-#pragma unroll
-                for(int e = 0; e < E; e++) u[e] *= p[e];
-            }
-#pragma unroll
-            for(int e = 0; e < E; e++) o[e] = fmaf(a.scale, u[e], o[e]);
-        }
-        if(a.out) R.store(static_cast<T*>(a.out) + r * a.ldo, o);
-        if(a.pre != B200RL_NORM_NONE){
+    for(int k = 0; k < 4; k++)
+        if(parameters[k]){
             float p[E];
-            normalise<Row<T, VEC, TPR, E>, TPR>(R, a.pre, o, a.epsilon, buffer, turn);
-            if(a.pre_weight){
-                R.parameters(a.pre_weight, 1.0f, p);
+            row.parameters(parameters[k], 0.0f, p);
 #pragma unroll
-                for(int e = 0; e < E; e++) o[e] *= p[e];
-            }
-            if(a.pre_bias){
-                R.parameters(a.pre_bias, 0.0f, p);
+            for(int i = 0; i < E / 4; i++) kept(k, i) = make_float4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
+        }
+    auto affine = [&](float2 (&v)[P], int weight, int bias){
+        if(parameters[weight])
 #pragma unroll
-                for(int e = 0; e < E; e++) o[e] += p[e];
+            for(int i = 0; i < E / 4; i++){
+                const float4 w = kept(weight, i);
+                v[2 * i] = mul2(v[2 * i], make_float2(w.x, w.y)); v[2 * i + 1] = mul2(v[2 * i + 1], make_float2(w.z, w.w));
             }
-            R.store(static_cast<T*>(a.normed) + r * a.ldn, o);
+        if(parameters[bias])
+#pragma unroll
+            for(int i = 0; i < E / 4; i++){
+                const float4 w = kept(bias, i);
+                v[2 * i] = add2(v[2 * i], make_float2(w.x, w.y)); v[2 * i + 1] = add2(v[2 * i + 1], make_float2(w.z, w.w));
+            }
+    };
+    typename R::Raw raw_r{}, raw_u{}, raw_gate{};                        // 0 where there is no such operand
+    long long gate_row = -1;
+    auto fetch = [&](long long r){
+        if(a.branch) row.fetch(a.branch, r * a.ldb, raw_u);
+        if(a.residual) row.fetch(a.residual, r * a.ldr, raw_r);
+        if(a.gate){
+            const long long g = a.gate_rows >= a.rows ? 0 : a.gate_rows == 1 ? r : (long long)((uint32_t)r / (uint32_t)a.gate_rows);
+            if(g != gate_row) row.fetch(a.gate, g * a.ldg, raw_gate);
+            gate_row = g;
+        }
+    };
+    constexpr bool AHEAD = VEC > 1;
+    const long long step = (long long)gridDim.x * ROWS;
+    long long r = (long long)blockIdx.x * ROWS + threadIdx.x / TPR;
+    if(AHEAD && r < a.rows) fetch(r);
+    for(; r < a.rows; r += step){
+        if(!AHEAD) fetch(r);
+        float2 o[P];
+        row.pairs(raw_r, o);
+        if(a.branch){
+            float2 u[P], gate[P];
+            row.pairs(raw_u, u);
+            if(a.gate) row.pairs(raw_gate, gate);
+            if(AHEAD && r + step < a.rows) fetch(r + step);
+            if(a.post != B200RL_NORM_NONE){
+                normalise<TPR>(row, a.post, u, a.epsilon, buffer, turn);
+                affine(u, 0, 1);
+            }
+            if(a.gate)
+#pragma unroll
+                for(int i = 0; i < P; i++) u[i] = mul2(u[i], gate[i]);
+#pragma unroll
+            for(int i = 0; i < P; i++) o[i] = fma2(both(a.scale), u[i], o[i]);
+        }
+        else if(AHEAD && r + step < a.rows) fetch(r + step);
+        if(a.out) row.store(a.out, r * a.ldo, o);
+        if(a.pre != B200RL_NORM_NONE){
+            normalise<TPR>(row, a.pre, o, a.epsilon, buffer, turn);
+            affine(o, 2, 3);
+            row.store(a.normed, r * a.ldn, o);
         }
     }
 }
 
-// q <- the gradient in front of a norm, from the gradient q of the normalised row: rstd (q - [mean q] - hat mean(q hat)); hat is the normalised row
-template <typename R, int TPR, int E>
-__device__ __forceinline__ void through_norm(const R& row, int kind, float (&q)[E], const float (&hat)[E], float rstd, float (*buffer)[2][TPR / 32], int& turn){
-    const float inv = 1.0f / (float)row.dim;
-    float s[2] = {0.0f, 0.0f};
-#pragma unroll
-    for(int e = 0; e < E; e++){ s[0] += q[e]; s[1] = fmaf(q[e], hat[e], s[1]); }
-    row_sums<TPR>(s, buffer, turn);
-    const float mean = kind == B200RL_NORM_LAYER ? s[0] * inv : 0.0f, along = s[1] * inv;
-#pragma unroll
-    for(int e = 0; e < E; e++) q[e] = row.inside(e) ? rstd * (q[e] - mean - hat[e] * along) : 0.0f;     // the next norm sums what lies behind the row's end too
-}
-
-// A worker (the threads of a row) takes rows_per_worker consecutive rows; the column sums of the parameter gradients stay in its registers.
-template <typename T, int VEC, int TPR, int E>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_backward_kernel(NormBackward a){
-    constexpr int WORKERS = TPR < 128 ? 128 / TPR : 1;
-    __shared__ float buffer1[2][1][TPR / 32], buffer2[2][2][TPR / 32];
-    int turn1 = 0, turn2 = 0;
+// ---- backward -----------------------------------------------------------------------------------------------------------------------------------------
+// A worker (the threads of a row) takes rows_per_worker consecutive rows. What a thread keeps over its rows -- its columns' parameters and the sums of their gradients -- lies
+// in shared memory at places of its own (registers for it would leave one CTA per multiprocessor); the next row's loads are under way while a row is summed. BIAS: sums for the
+// biases too, and the post norm's bias, which the gate's gradient sees.
+template <int TPR, int E, bool BIAS, bool GATE> struct Kept {
+    enum { PRE_WEIGHT, POST_WEIGHT, SUM_POST_WEIGHT, SUM_PRE_WEIGHT, SUM_POST_BIAS, SUM_PRE_BIAS = SUM_POST_BIAS + (BIAS ? 1 : 0), SUM_GATE = SUM_PRE_BIAS + (BIAS ? 1 : 0),
+           COUNT = SUM_GATE + (GATE ? 1 : 0) };
+    static constexpr int worker_bytes = COUNT * E * TPR * 4;
+    static_assert(worker_bytes + 1024 <= 232448, "rows of B200RL_NORM_MAX_DIM elements fit");
+    float4* mine;                                            // [COUNT][E / 4][TPR]
+    __device__ __forceinline__ float4& at(int array, int quad){ return mine[(array * (E / 4) + quad) * TPR]; }
+};
+template <typename T, int VEC, int TPR, int E, bool BIAS, bool GATE>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 3 : TPR == 128 ? 4 : TPR == 256 ? 2 : 1) norm_backward_kernel(NormBackward a){
+    constexpr int WORKERS = TPR < 128 ? 128 / TPR : 1, P = E / 2;
+    using R = Row<T, VEC, TPR, E>;
+    using K = Kept<TPR, E, BIAS, GATE>;
+    extern __shared__ __align__(16) float4 kept_memory[];
+    __shared__ __align__(16) float buffer[2][4][TPR / 32];
+    after_predecessor();
+    int turn = 0;
     const int worker = blockIdx.x * WORKERS + threadIdx.x / TPR;
     const long long first = (long long)worker * a.rows_per_worker, last = min((long long)a.rows, first + a.rows_per_worker);
     if(first >= last) return;                                // a whole row's threads leave together
-    const Row<T, VEC, TPR, E> R{(int)(threadIdx.x % TPR), a.dim};
-    float sum[SUMS][E], d_gate[E];
+    const R row{(int)(threadIdx.x % TPR), a.dim};
+    K kept{kept_memory + (threadIdx.x / TPR) * (K::worker_bytes / 16) + threadIdx.x % TPR};
+    const bool gated = GATE && a.gate;                       // the form for rows at odd addresses is built once, with everything in it
+    const bool pre = a.pre != B200RL_NORM_NONE, post = a.post != B200RL_NORM_NONE, layer = a.pre == B200RL_NORM_LAYER || a.post == B200RL_NORM_LAYER;
+    const float inv = 1.0f / (float)a.dim;
+    {
+        float p[E];
+        auto keep = [&](int array){
 #pragma unroll
-    for(int e = 0; e < E; e++){
-        d_gate[e] = 0.0f;
+            for(int i = 0; i < E / 4; i++) kept.at(array, i) = make_float4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
+        };
+        row.parameters(a.pre_weight, 1.0f, p);
+        keep(K::PRE_WEIGHT);
+        row.parameters(a.post_weight, 1.0f, p);
+        keep(K::POST_WEIGHT);
 #pragma unroll
-        for(int i = 0; i < SUMS; i++) sum[i][e] = 0.0f;
+        for(int e = 0; e < E; e++) p[e] = 0.0f;
+        keep(K::SUM_POST_WEIGHT);
+        keep(K::SUM_PRE_WEIGHT);
+        if constexpr(BIAS){ keep(K::SUM_POST_BIAS); keep(K::SUM_PRE_BIAS); }
+        if constexpr(GATE) keep(K::SUM_GATE);
     }
-    for(long long r = first; r < last; r++){
-        float d[E], u[E];
-        if(a.d_out) R.load(static_cast<const T*>(a.d_out) + r * a.lddo, d);
-        else
+    // array += a b for the pairs 2 i, 2 i + 1
+    auto add_to = [&](int array, int i, float2 a0, float2 b0, float2 a1, float2 b1){
+        float4 v = kept.at(array, i);
+        const float2 lo = fma2(a0, b0, make_float2(v.x, v.y)), hi = fma2(a1, b1, make_float2(v.z, v.w));
+        kept.at(array, i) = make_float4(lo.x, lo.y, hi.x, hi.y);
+    };
+    auto hand_out = [&](int array, float (&v)[E]){
 #pragma unroll
-            for(int e = 0; e < E; e++) d[e] = 0.0f;
-        if(a.branch) R.load(static_cast<const T*>(a.branch) + r * a.ldb, u);
-        if(a.pre != B200RL_NORM_NONE){
-            float x[E], q[E], p[E];
-            R.load(static_cast<const T*>(a.d_normed) + r * a.lddn, q);
-            R.load(static_cast<const T*>(a.out) + r * a.ldo, x);
-            const float rstd = normalise<Row<T, VEC, TPR, E>, TPR>(R, a.pre, x, a.epsilon, buffer1, turn1);
-            R.parameters(a.pre_weight, 1.0f, p);
-#pragma unroll
-            for(int e = 0; e < E; e++){
-                sum[2][e] = fmaf(q[e], x[e], sum[2][e]);
-                sum[3][e] += q[e];
-                q[e] *= p[e];
-            }
-            through_norm<Row<T, VEC, TPR, E>, TPR>(R, a.pre, q, x, rstd, buffer2, turn2);
-#pragma unroll
-            for(int e = 0; e < E; e++) d[e] += q[e];
+        for(int i = 0; i < E / 4; i++){ const float4 q = kept.at(array, i); v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w; }
+    };
+    // the group of rows that share a gate row: of the row that is fetched, and (one row behind) of the row that is summed
+    long long group = -1, group_end = first;
+    if(gated){
+        group = first / a.gate_rows;
+        group_end = min((long long)a.rows, (group + 1) * a.gate_rows);
+    }
+    long long sum_group = group, sum_begin = group * a.gate_rows, sum_end = group_end;
+    typename R::Raw raw_d{}, raw_u{}, raw_q{}, raw_x{}, raw_gate{};      // 0 where there is no such operand
+    auto fetch = [&](long long r){
+        if(a.d_out) row.fetch(a.d_out, r * a.lddo, raw_d);
+        if(a.branch) row.fetch(a.branch, r * a.ldb, raw_u);
+        if(pre){ row.fetch(a.d_normed, r * a.lddn, raw_q); row.fetch(a.out, r * a.ldo, raw_x); }
+        if(gated && r == group_end){                         // the first row of the next group
+            group++;
+            group_end = min((long long)a.rows, group_end + a.gate_rows);
+            row.fetch(a.gate, group * a.ldg, raw_gate);
         }
-        if(a.d_residual) R.store(static_cast<T*>(a.d_residual) + r * a.lddr, d);
-        if(!a.branch) continue;
+    };
+    constexpr bool AHEAD = VEC > 1;
+    if(gated) row.fetch(a.gate, group * a.ldg, raw_gate);
+    if(AHEAD) fetch(first);
+    for(long long r = first; r < last; r++){
+        float2 d[P], u[P], x[P], q[P], gate[GATE ? P : 1];
+        if(!AHEAD) fetch(r);
+        row.pairs(raw_d, d); row.pairs(raw_u, u); row.pairs(raw_x, x); row.pairs(raw_q, q);
+        if constexpr(GATE) row.pairs(raw_gate, gate);
+        if(AHEAD && r + 1 < last) fetch(r + 1);
+        // the statistics of both norms with the same barriers: means about the first elements, then squares
+        if(layer){
+            float start[2] = {x[0].x, u[0].x}, s[2] = {0.0f, 0.0f};
+            row_first<TPR>(start);
+            if(a.pre != B200RL_NORM_LAYER) start[0] = 0.0f;
+            if(a.post != B200RL_NORM_LAYER) start[1] = 0.0f;
 #pragma unroll
-        for(int e = 0; e < E; e++) d[e] *= a.scale;          // from here on the gradient of gate u
-        float rstd = 0.0f, hat[E];
-        if(a.post != B200RL_NORM_NONE) rstd = normalise<Row<T, VEC, TPR, E>, TPR>(R, a.post, u, a.epsilon, buffer1, turn1);
+            for(int i = 0; i < P; i++){ x[i] = add2(x[i], both(-start[0])); u[i] = add2(u[i], both(-start[1])); }
+            row.clear_outside(x); row.clear_outside(u);
 #pragma unroll
-        for(int e = 0; e < E; e++) hat[e] = u[e];
-        float w[E];
-        if(a.post != B200RL_NORM_NONE) R.parameters(a.post_weight, 1.0f, w);
-        if(a.gate){
-            float p[E];
-            if(a.d_gate){
-                if(a.post != B200RL_NORM_NONE){
-                    R.parameters(a.post_bias, 0.0f, p);
+            for(int i = 0; i < P; i++){ s[0] += across(x[i]); s[1] += across(u[i]); }
+            row_sums<TPR>(s, buffer, turn);
+            const float mean_x = a.pre == B200RL_NORM_LAYER ? s[0] * inv : 0.0f, mean_u = a.post == B200RL_NORM_LAYER ? s[1] * inv : 0.0f;
 #pragma unroll
-                    for(int e = 0; e < E; e++) u[e] = fmaf(hat[e], w[e], p[e]);
+            for(int i = 0; i < P; i++){ x[i] = add2(x[i], both(-mean_x)); u[i] = add2(u[i], both(-mean_u)); }
+            row.clear_outside(x); row.clear_outside(u);
+        }
+        float rstd_u = 1.0f;
+        {
+            // squares of both rows; the sums of the pre norm's gradient g = q weight go with them: sum g hat = rstd sum g x
+            float2 xx = both(0.0f), uu = xx, gg = xx, gx = xx;
+#pragma unroll
+            for(int i = 0; i < E / 4; i++){
+                const float4 w = kept.at(K::PRE_WEIGHT, i);
+                const float2 g0 = mul2(q[2 * i], make_float2(w.x, w.y)), g1 = mul2(q[2 * i + 1], make_float2(w.z, w.w));
+                xx = fma2(x[2 * i], x[2 * i], xx); xx = fma2(x[2 * i + 1], x[2 * i + 1], xx);
+                uu = fma2(u[2 * i], u[2 * i], uu); uu = fma2(u[2 * i + 1], u[2 * i + 1], uu);
+                gg = add2(gg, add2(g0, g1));
+                gx = fma2(g0, x[2 * i], gx); gx = fma2(g1, x[2 * i + 1], gx);
+            }
+            float s[4] = {across(xx), across(uu), across(gg), across(gx)};
+            row_sums<TPR>(s, buffer, turn);
+            if(pre){
+                const float rstd = 1.0f / sqrtf(s[0] * inv + a.epsilon), mean = a.pre == B200RL_NORM_LAYER ? s[2] * inv : 0.0f, along = s[3] * rstd * inv;
+#pragma unroll
+                for(int i = 0; i < E / 4; i++){
+                    const float4 w = kept.at(K::PRE_WEIGHT, i);
+                    const float2 h0 = mul2(x[2 * i], both(rstd)), h1 = mul2(x[2 * i + 1], both(rstd)), q0 = q[2 * i], q1 = q[2 * i + 1];
+                    add_to(K::SUM_PRE_WEIGHT, i, q0, h0, q1, h1);
+                    if constexpr(BIAS) add_to(K::SUM_PRE_BIAS, i, q0, both(1.0f), q1, both(1.0f));
+                    d[2 * i] = fma2(fma2(h0, both(-along), fma2(q0, make_float2(w.x, w.y), both(-mean))), both(rstd), d[2 * i]);
+                    d[2 * i + 1] = fma2(fma2(h1, both(-along), fma2(q1, make_float2(w.z, w.w), both(-mean))), both(rstd), d[2 * i + 1]);
                 }
+                if(a.pre == B200RL_NORM_LAYER) row.clear_outside(d);     // the post norm sums what lies behind the row's end too
+            }
+            if(post) rstd_u = 1.0f / sqrtf(s[1] * inv + a.epsilon);
+        }
+        if(a.d_residual) row.store(a.d_residual, r * a.lddr, d);
+        if(!a.branch) continue;
+        // d: from here on the gradient of gate u; u: the normalised row
 #pragma unroll
-                for(int e = 0; e < E; e++) d_gate[e] = fmaf(d[e], u[e], d_gate[e]);
-                const long long g = r / a.gate_rows, begin = g * a.gate_rows;
-                const bool ends = r + 1 == a.rows || (r + 1) % a.gate_rows == 0;
+        for(int i = 0; i < P; i++){ d[i] = mul2(d[i], both(a.scale)); u[i] = mul2(u[i], both(rstd_u)); }
+        if constexpr(GATE) if(gated){
+            if(a.d_gate){
+                float b[E];
+                if(BIAS && post) row.parameters(a.post_bias, 0.0f, b);
+#pragma unroll
+                for(int i = 0; i < E / 4; i++){
+                    float2 v0 = u[2 * i], v1 = u[2 * i + 1];
+                    if(post){
+                        const float4 w = kept.at(K::POST_WEIGHT, i);
+                        v0 = fma2(v0, make_float2(w.x, w.y), BIAS ? make_float2(b[4 * i], b[4 * i + 1]) : both(0.0f));
+                        v1 = fma2(v1, make_float2(w.z, w.w), BIAS ? make_float2(b[4 * i + 2], b[4 * i + 3]) : both(0.0f));
+                    }
+                    add_to(K::SUM_GATE, i, d[2 * i], v0, d[2 * i + 1], v1);
+                }
+                const bool ends = r + 1 == sum_end;
                 if(ends || r + 1 == last){
                     // the gate row's sum is complete here, or a piece of it: the group's rows go on with the next worker, or began with one before
-                    if(ends && begin >= first) R.store(static_cast<T*>(a.d_gate) + g * a.lddg, d_gate);
+                    float sum[E];
+                    hand_out(K::SUM_GATE, sum);
+                    if(ends && sum_begin >= first) row.store(a.d_gate, sum_group * a.lddg, sum);
                     else{
-                        float* piece = a.pieces + ((long long)worker * 2 + (begin >= first ? 1 : 0)) * a.dim;
+                        float* piece = a.pieces + ((long long)worker * 2 + (sum_begin >= first ? 1 : 0)) * a.dim;
 #pragma unroll
-                        for(int e = 0; e < E; e++) if(R.inside(e)) piece[R.column(e / VEC) + e % VEC] = d_gate[e];
+                        for(int e = 0; e < E; e++) if(row.inside(e)) piece[row.column(e / VEC) + e % VEC] = sum[e];
                     }
 #pragma unroll
-                    for(int e = 0; e < E; e++) d_gate[e] = 0.0f;
+                    for(int i = 0; i < E / 4; i++) kept.at(K::SUM_GATE, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    sum_group++; sum_begin = sum_end; sum_end = min((long long)a.rows, sum_end + a.gate_rows);
                 }
             }
-            R.load(static_cast<const T*>(a.gate) + r / a.gate_rows * a.ldg, p);
 #pragma unroll
-            for(int e = 0; e < E; e++) d[e] *= p[e];
+            for(int i = 0; i < P; i++) d[i] = mul2(d[i], gate[i]);
         }
-        if(a.post != B200RL_NORM_NONE){
+        if(post){
+            float2 gg = both(0.0f), gh = gg;
 #pragma unroll
-            for(int e = 0; e < E; e++){
-                sum[0][e] = fmaf(d[e], hat[e], sum[0][e]);
-                sum[1][e] += d[e];
-                d[e] *= w[e];
+            for(int i = 0; i < E / 4; i++){
+                const float4 w = kept.at(K::POST_WEIGHT, i);
+                add_to(K::SUM_POST_WEIGHT, i, d[2 * i], u[2 * i], d[2 * i + 1], u[2 * i + 1]);
+                if constexpr(BIAS) add_to(K::SUM_POST_BIAS, i, d[2 * i], both(1.0f), d[2 * i + 1], both(1.0f));
+                d[2 * i] = mul2(d[2 * i], make_float2(w.x, w.y));
+                d[2 * i + 1] = mul2(d[2 * i + 1], make_float2(w.z, w.w));
+                gg = add2(gg, add2(d[2 * i], d[2 * i + 1]));
+                gh = fma2(d[2 * i], u[2 * i], gh); gh = fma2(d[2 * i + 1], u[2 * i + 1], gh);
             }
-            through_norm<Row<T, VEC, TPR, E>, TPR>(R, a.post, d, hat, rstd, buffer2, turn2);
+            float s[2] = {across(gg), across(gh)};
+            row_sums<TPR>(s, buffer, turn);
+            const float mean = a.post == B200RL_NORM_LAYER ? s[0] * inv : 0.0f, along = s[1] * inv;
+#pragma unroll
+            for(int i = 0; i < P; i++) d[i] = mul2(fma2(u[i], both(-along), add2(d[i], both(-mean))), both(rstd_u));
         }
-        if(a.d_branch) R.store(static_cast<T*>(a.d_branch) + r * a.lddb, d);
+        if(a.d_branch) row.store(a.d_branch, r * a.lddb, d);
     }
+    constexpr int sums[SUMS] = {K::SUM_POST_WEIGHT, K::SUM_POST_BIAS, K::SUM_PRE_WEIGHT, K::SUM_PRE_BIAS};
 #pragma unroll
     for(int i = 0; i < SUMS; i++)
-        if(a.d_params[i]){
+        if(a.d_params[i] && (BIAS || i % 2 == 0)){
+            float sum[E];
+            hand_out(sums[i], sum);
             float* partial = a.partials + ((long long)i * a.workers + worker) * a.dim;
 #pragma unroll
-            for(int e = 0; e < E; e++) if(R.inside(e)) partial[R.column(e / VEC) + e % VEC] = sum[i][e];
+            for(int e = 0; e < E; e++) if(row.inside(e)) partial[row.column(e / VEC) + e % VEC] = sum[e];
         }
 }
 
-// The sums over the workers, in their order: blockIdx.y < SUMS the parameter gradients, behind them the gate rows that begin with worker blockIdx.y - SUMS and go on
-// with the next. 32 columns a CTA, eight threads a column.
+// A gate row whose rows lie with more than one worker: its pieces are those of workers first .. first + n - 1 (slot 1 of the first, which it goes beyond, slot 0 of the others).
+struct GatePieces { long long group; int first, n; };
+__device__ __forceinline__ GatePieces gate_pieces(const NormBackward& a, long long group){
+    const long long begin = group * a.gate_rows, end = min((long long)a.rows, begin + a.gate_rows);
+    const int w = (int)(begin / a.rows_per_worker);
+    return {group, w, (int)((end - 1) / a.rows_per_worker) - w + 1};
+}
+
+// The sums over the workers, in their order: blockIdx.y < SUMS the parameter gradients, behind them gate rows (few, of many pieces). 32 columns a CTA, 32 threads a column.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_backward_sums_kernel(NormBackward a){
-    __shared__ float shared[8][33];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
-    const float* part; long long stride; int n;
-    long long g = 0;
-    if(blockIdx.y < SUMS){
+__global__ void __launch_bounds__(1024) norm_backward_sums_kernel(NormBackward a){
+    __shared__ float shared[32][33];
+    after_predecessor();
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    const bool parameter = blockIdx.y < SUMS;
+    const float* part; long long stride; int n, skip = 0;
+    GatePieces g{};
+    if(parameter){
         if(!a.d_params[blockIdx.y]) return;
         part = a.partials + (long long)blockIdx.y * a.workers * a.dim; stride = a.dim; n = a.workers;
     }
     else{
-        const long long w = blockIdx.y - SUMS, next = (w + 1) * a.rows_per_worker;      // the next worker's first row
-        g = next / a.gate_rows;
-        const long long begin = g * a.gate_rows;
-        if(begin == next || begin < w * a.rows_per_worker) return;                       // a gate row begins there, or began with an earlier worker
-        const long long end = min((long long)a.rows, begin + a.gate_rows);
-        n = (int)((end - 1) / a.rows_per_worker - w) + 1;
-        part = a.pieces + w * 2 * a.dim; stride = 2ll * a.dim;
+        g = gate_pieces(a, blockIdx.y - SUMS);
+        if(g.n == 1) return;
+        part = a.pieces + 2ll * g.first * a.dim; stride = 2ll * a.dim; n = g.n; skip = a.dim;
     }
     float v = 0.0f;
     if(c < a.dim)
-        for(int i = slice; i < n; i += 8) v += part[i * stride + (blockIdx.y >= SUMS && i == 0 ? a.dim : 0) + c];
-    shared[slice][threadIdx.x & 31] = v;
+#pragma unroll 4
+        for(int i = slice; i < n; i += 32) v += part[i * stride + (i == 0 ? skip : 0) + c];
+    shared[slice][lane] = v;
     __syncthreads();
-    if(slice || c >= a.dim) return;
+    // a warp a column: its 32 slices, summed in a fixed tree
+    v = shared[lane][slice];
 #pragma unroll
-    for(int i = 1; i < 8; i++) v += shared[i][threadIdx.x];
-    if(blockIdx.y < SUMS) a.d_params[blockIdx.y][c] = a.accumulate ? a.d_params[blockIdx.y][c] + v : v;
-    else static_cast<T*>(a.d_gate)[g * a.lddg + c] = from_float<T>(v);
+    for(int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int column = blockIdx.x * 32 + slice;
+    if(lane || column >= a.dim) return;
+    if(parameter) a.d_params[blockIdx.y][column] = a.accumulate ? a.d_params[blockIdx.y][column] + v : v;
+    else static_cast<T*>(a.d_gate)[g.group * a.lddg + column] = from_float<T>(v);
+}
+// The same for many gate rows of few pieces: blockIdx.y is the worker behind a boundary, a thread a column.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_backward_gates_kernel(NormBackward a){
+    after_predecessor();
+    const long long row = (blockIdx.y + 1ll) * a.rows_per_worker;                   // the worker's first row
+    const GatePieces g = gate_pieces(a, row / a.gate_rows);
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if(c >= a.dim || g.first != (int)blockIdx.y) return;                            // a gate row begins at the boundary, or its first boundary is an earlier one
+    float v = a.pieces[(2ll * g.first + 1) * a.dim + c];
+    for(int i = 1; i < g.n; i++) v += a.pieces[2ll * (g.first + i) * a.dim + c];
+    static_cast<T*>(a.d_gate)[g.group * a.lddg + c] = from_float<T>(v);
 }
 
-// threads and elements per thread that hold a row
-template <typename F>
+template <int TPR, int E> struct Shape { static constexpr int tpr = TPR, e = E; };
+// Threads and elements per thread that hold a row: 16 elements a thread, 8 of fp32, so that the raw row that is under way takes the same registers either way
+template <typename T, typename F>
 static int dispatch_row(int dim, F f){
-    if(dim <= 32 * 8) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 8>{});
-    if(dim <= 32 * 16) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 16>{});
-    if(dim <= 128 * 8) return f(std::integral_constant<int, 128>{}, std::integral_constant<int, 8>{});
-    if(dim <= 128 * 16) return f(std::integral_constant<int, 128>{}, std::integral_constant<int, 16>{});
-    if(dim <= 512 * 8) return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 8>{});
-    return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 16>{});
+    constexpr int E = sizeof(T) == 4 ? 8 : 16;
+    if(dim <= 32 * E) return f(Shape<32, E>{});
+    if(dim <= 128 * E) return f(Shape<128, E>{});
+    if(dim <= 256 * E) return f(Shape<256, E>{});
+    if constexpr(E == 8) if(dim > 512 * E) return f(Shape<1024, E>{});
+    return f(Shape<512, E>{});
 }
 
-// workers of the backward pass and the consecutive rows that each takes
+// Workers of the backward pass and the consecutive rows that each takes: what is resident at once (rows of up to 512 elements: 12 workers a multiprocessor, and so on), a row
+// each where there are fewer rows than that, then four, so that the sums over the workers stay small against the rows.
 static void plan_workers(int rows, int dim, int* workers, int* rows_per_worker){
-    const int most = NUM_SMS * (dim <= 512 ? 16 : dim <= 2048 ? 4 : 1);
-    const int per = rows <= 4 * most ? (rows <= most ? 1 : 4) : (rows + most - 1) / most;
+    const int most = NUM_SMS * (dim <= 512 ? 12 : dim <= 2048 ? 4 : dim <= 4096 ? 2 : 1);
+    const int per = rows <= 4 * most ? (rows <= most ? 1 : 4) : (rows - 1) / most + 1;
     *rows_per_worker = per;
-    *workers = (rows + per - 1) / per;
+    *workers = (rows - 1) / per + 1;
+}
+
+template <typename T, int VEC, int TPR, int E>
+static int launch_forward(const NormForward& a, cudaStream_t s){
+    auto* kernel = norm_forward_kernel<T, VEC, TPR, E>;
+    constexpr int ROWS = TPR < 128 ? 128 / TPR : 1, THREADS = TPR < 128 ? 128 : TPR, each = ROWS * E * TPR * 4;
+    static_assert(4 * each + 1024 <= 232448, "four parameters of B200RL_NORM_MAX_DIM elements fit");
+    const int bytes = each * ((a.post_weight != nullptr) + (a.post_bias != nullptr) + (a.pre_weight != nullptr) + (a.pre_bias != nullptr));
+    static std::atomic<int> resident[MAX_DEVICES][5];        // CTAs a multiprocessor, by the number of parameters: 0 until looked up
+    int dev = 0;
+    const int rc = current_device(&dev);
+    if(rc) return rc;
+    int n = resident[dev][bytes / each].load(std::memory_order_acquire);
+    if(n == 0){
+        B200RL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * each));
+        B200RL_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, THREADS, bytes));
+        if(n < 1) return B200RL_ERR_UNSUPPORTED;
+        resident[dev][bytes / each].store(n, std::memory_order_release);
+    }
+    const int most = NUM_SMS * n, ctas = (a.rows - 1) / ROWS + 1;
+    B200RL_CUDA_TRY(launch_after(kernel, dim3(ctas < most ? ctas : most), dim3(THREADS), bytes, s, a));
+    return B200RL_OK;
+}
+
+template <typename T, int VEC, int TPR, int E, bool BIAS, bool GATE>
+static int launch_backward(const NormBackward& a, cudaStream_t s){
+    auto* kernel = norm_backward_kernel<T, VEC, TPR, E, BIAS, GATE>;
+    constexpr int WORKERS = TPR < 128 ? 128 / TPR : 1, bytes = WORKERS * Kept<TPR, E, BIAS, GATE>::worker_bytes;
+    static std::atomic<bool> configured[MAX_DEVICES];
+    int dev = 0;
+    const int rc = current_device(&dev);
+    if(rc) return rc;
+    if(!configured[dev].load(std::memory_order_acquire)){
+        B200RL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        configured[dev].store(true, std::memory_order_release);
+    }
+    B200RL_CUDA_TRY(launch_after(kernel, dim3((a.workers + WORKERS - 1) / WORKERS), dim3(TPR < 128 ? 128 : TPR), bytes, s, a));
+    return B200RL_OK;
 }
 
 }  // namespace b200rl
@@ -378,14 +612,12 @@ int b200rl_norm_residual_forward(int type, int post, const float* post_weight, c
     const int n = 16 / (int)e;
     const bool vector = dim % n == 0 && (!branch || rows_aligned(branch, a.ldb, e)) && (!gate || rows_aligned(gate, a.ldg, e)) &&
                         (!residual || rows_aligned(residual, a.ldr, e)) && (!out || rows_aligned(out, a.ldo, e)) && (!normed || rows_aligned(normed, a.ldn, e));
-    return dispatch_row(dim, [&](auto tpr, auto el){
-        constexpr int TPR = decltype(tpr)::value, E = decltype(el)::value, ROWS = TPR < 128 ? 128 / TPR : 1, THREADS = TPR < 128 ? 128 : TPR;
-        const int grid = (rows - 1) / ROWS + 1;
-        B200RL_DISPATCH_TYPE(type, if(vector) norm_forward_kernel<T, 16 / sizeof(T), TPR, E><<<grid, THREADS, 0, (cudaStream_t)stream>>>(a);
-                                   else norm_forward_kernel<T, 1, TPR, E><<<grid, THREADS, 0, (cudaStream_t)stream>>>(a))
-        B200RL_LAUNCH_CHECK("norm_residual_forward");
-        return B200RL_OK;
-    });
+    int rc = B200RL_ERR_UNSUPPORTED;
+    B200RL_DISPATCH_TYPE(type, rc = dispatch_row<T>(dim, [&](auto shape){
+        constexpr int TPR = decltype(shape)::tpr, E = decltype(shape)::e;
+        return vector ? launch_forward<T, 16 / sizeof(T), TPR, E>(a, (cudaStream_t)stream) : launch_forward<T, 1, TPR, E>(a, (cudaStream_t)stream);
+    }))
+    return rc;
 }
 
 size_t b200rl_norm_residual_backward_scratch_bytes(int rows, int dim){
@@ -430,20 +662,24 @@ int b200rl_norm_residual_backward(int type, int post, const float* post_weight, 
     const bool vector = dim % n == 0 && (!branch || rows_aligned(branch, a.ldb, e)) && (!gate || rows_aligned(gate, a.ldg, e)) && (pre == B200RL_NORM_NONE || rows_aligned(out, a.ldo, e)) &&
                         (!d_out || rows_aligned(d_out, a.lddo, e)) && (!d_normed || rows_aligned(d_normed, a.lddn, e)) && (!d_branch || rows_aligned(d_branch, a.lddb, e)) &&
                         (!d_residual || rows_aligned(d_residual, a.lddr, e)) && (!d_gate || rows_aligned(d_gate, a.lddg, e));
-    const int rc = dispatch_row(dim, [&](auto tpr, auto el){
-        constexpr int TPR = decltype(tpr)::value, E = decltype(el)::value, WORKERS = TPR < 128 ? 128 / TPR : 1, THREADS = TPR < 128 ? 128 : TPR;
-        const int grid = (a.workers + WORKERS - 1) / WORKERS;
-        B200RL_DISPATCH_TYPE(type, if(vector) norm_backward_kernel<T, 16 / sizeof(T), TPR, E><<<grid, THREADS, 0, (cudaStream_t)stream>>>(a);
-                                   else norm_backward_kernel<T, 1, TPR, E><<<grid, THREADS, 0, (cudaStream_t)stream>>>(a))
-        B200RL_LAUNCH_CHECK("norm_residual_backward");
-        return B200RL_OK;
-    });
+    const bool bias = d_post_bias || d_pre_bias || (post_bias && gate);
+    int rc = B200RL_ERR_UNSUPPORTED;
+    B200RL_DISPATCH_TYPE(type, rc = dispatch_row<T>(dim, [&](auto shape){
+        constexpr int TPR = decltype(shape)::tpr, E = decltype(shape)::e, V = 16 / sizeof(T);
+        const cudaStream_t st = (cudaStream_t)stream;
+        if(!vector) return launch_backward<T, 1, TPR, E, true, true>(a, st);
+        if(bias) return gate ? launch_backward<T, V, TPR, E, true, true>(a, st) : launch_backward<T, V, TPR, E, true, false>(a, st);
+        return gate ? launch_backward<T, V, TPR, E, false, true>(a, st) : launch_backward<T, V, TPR, E, false, false>(a, st);
+    }))
     if(rc) return rc;
-    const bool shared_gates = d_gate && a.workers > 1;
-    if(shared_gates || d_post_weight || d_post_bias || d_pre_weight || d_pre_bias){
-        const dim3 grid((dim + 31) / 32, SUMS + (shared_gates ? a.workers - 1 : 0));
-        B200RL_DISPATCH_TYPE(type, norm_backward_sums_kernel<T><<<grid, 256, 0, (cudaStream_t)stream>>>(a))
-        B200RL_LAUNCH_CHECK("norm_residual_backward sums");
+    const bool shared_gates = d_gate && a.workers > 1 && gate_rows > 1, few_gates = shared_gates && gates <= 32;
+    if(few_gates || d_post_weight || d_post_bias || d_pre_weight || d_pre_bias){
+        const dim3 grid((dim + 31) / 32, SUMS + (few_gates ? gates : 0));
+        B200RL_DISPATCH_TYPE(type, B200RL_CUDA_TRY(launch_after(norm_backward_sums_kernel<T>, grid, dim3(1024), 0, (cudaStream_t)stream, a)))
+    }
+    if(shared_gates && !few_gates){
+        const dim3 grid((dim + 255) / 256, a.workers - 1);
+        B200RL_DISPATCH_TYPE(type, B200RL_CUDA_TRY(launch_after(norm_backward_gates_kernel<T>, grid, dim3(256), 0, (cudaStream_t)stream, a)))
     }
     return B200RL_OK;
 }
