@@ -15,6 +15,24 @@ static_assert(ROW_THREADS_MAX * ELEMENTS_MAX == B200RL_NORM_MAX_DIM);
 constexpr int SUMS = 4;                                      // parameter gradients: post weight, post bias, pre weight, pre bias
 }
 
+// Threads and elements per thread that hold a row of T: up to 16 elements a thread, 8 of fp32, so that the raw row that is under way takes the same registers either way.
+template <int TPR, int E> struct Shape { static constexpr int tpr = TPR, e = E; };
+template <typename T, typename F>
+static int dispatch_row(int dim, F f){
+    if(dim <= 256) return f(Shape<32, 8>{});
+    if constexpr(sizeof(T) == 2) if(dim <= 512) return f(Shape<32, 16>{});
+    if(dim <= 1024) return f(Shape<128, 8>{});
+    if constexpr(sizeof(T) == 2) if(dim <= 2048) return f(Shape<128, 16>{});
+    if constexpr(sizeof(T) == 2) return dim <= 4096 ? f(Shape<256, 16>{}) : f(Shape<512, 16>{});
+    if(dim <= 2048) return f(Shape<256, 8>{});
+    return dim <= 4096 ? f(Shape<512, 8>{}) : f(Shape<1024, 8>{});
+}
+// CTAs of the backward pass on a multiprocessor, which leaves a thread 64 to 168 registers
+template <typename T> __host__ __device__ constexpr int backward_ctas(int tpr, int e){
+    const bool narrow = sizeof(T) == 2;
+    return tpr == 32 ? (narrow && e == 8 ? 5 : 3) : tpr == 128 ? (narrow && e == 8 ? 5 : 4) : tpr == 256 ? 2 : 1;
+}
+
 struct NormForward {
     const void* branch; long long ldb;
     const void* gate; long long ldg; int gate_rows;
@@ -39,6 +57,7 @@ struct NormBackward {
     float* d_params[SUMS];                                   // post weight, post bias, pre weight, pre bias (NULL: not asked for)
     float* partials;                                         // [SUMS][workers][dim]
     float* pieces;                                           // [workers][2][dim]: gate rows whose rows lie with more than one worker
+    int sums[SUMS], n_sums;                                  // those of d_params that are there
     int post, pre, rows, dim, workers, rows_per_worker, accumulate;
     float scale, epsilon;
 };
@@ -114,6 +133,15 @@ struct Row {
     __device__ __forceinline__ void clear_outside(float2 (&v)[E / 2]) const {
 #pragma unroll
         for(int i = 0; i < E / 2; i++){ if(!inside(2 * i)) v[i].x = 0.0f; if(!inside(2 * i + 1)) v[i].y = 0.0f; }
+    }
+    __device__ __forceinline__ void store_sums(float* p, const float (&v)[E]) const {
+#pragma unroll
+        for(int e = 0; e < E; e += VEC > 1 ? 4 : 1)
+            if(inside(e)){
+                float* at = p + column(e / VEC) + e % VEC;
+                if constexpr(VEC > 1) *reinterpret_cast<float4*>(at) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                else *at = v[e];
+            }
     }
     __device__ __forceinline__ void store(void* base, long long at, const float2 (&v)[E / 2]) const {
         float f[E];
@@ -290,7 +318,7 @@ template <int TPR, int E, bool BIAS, bool GATE> struct Kept {
     __device__ __forceinline__ float4& at(int array, int quad){ return mine[(array * (E / 4) + quad) * TPR]; }
 };
 template <typename T, int VEC, int TPR, int E, bool BIAS, bool GATE>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 3 : TPR == 128 ? 4 : TPR == 256 ? 2 : 1) norm_backward_kernel(NormBackward a){
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, backward_ctas<T>(TPR, E)) norm_backward_kernel(NormBackward a){
     constexpr int WORKERS = TPR < 128 ? 128 / TPR : 1, P = E / 2;
     using R = Row<T, VEC, TPR, E>;
     using K = Kept<TPR, E, BIAS, GATE>;
@@ -333,32 +361,25 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 3 : TPR == 
 #pragma unroll
         for(int i = 0; i < E / 4; i++){ const float4 q = kept.at(array, i); v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w; }
     };
-    // the group of rows that share a gate row: of the row that is fetched, and (one row behind) of the row that is summed
-    long long group = -1, group_end = first;
+    long long group = 0, group_begin = 0, group_end = 0;     // rows that share a gate row
     if(gated){
         group = first / a.gate_rows;
-        group_end = min((long long)a.rows, (group + 1) * a.gate_rows);
+        group_begin = group * a.gate_rows;
+        group_end = min((long long)a.rows, group_begin + a.gate_rows);
     }
-    long long sum_group = group, sum_begin = group * a.gate_rows, sum_end = group_end;
     typename R::Raw raw_d{}, raw_u{}, raw_q{}, raw_x{}, raw_gate{};      // 0 where there is no such operand
     auto fetch = [&](long long r){
         if(a.d_out) row.fetch(a.d_out, r * a.lddo, raw_d);
         if(a.branch) row.fetch(a.branch, r * a.ldb, raw_u);
         if(pre){ row.fetch(a.d_normed, r * a.lddn, raw_q); row.fetch(a.out, r * a.ldo, raw_x); }
-        if(gated && r == group_end){                         // the first row of the next group
-            group++;
-            group_end = min((long long)a.rows, group_end + a.gate_rows);
-            row.fetch(a.gate, group * a.ldg, raw_gate);
-        }
     };
-    constexpr bool AHEAD = VEC > 1;
+    constexpr bool AHEAD = VEC > 1 || sizeof(T) == 4;        // single 16-bit elements would take a register each
     if(gated) row.fetch(a.gate, group * a.ldg, raw_gate);
     if(AHEAD) fetch(first);
     for(long long r = first; r < last; r++){
-        float2 d[P], u[P], x[P], q[P], gate[GATE ? P : 1];
+        float2 d[P], u[P], x[P], q[P];
         if(!AHEAD) fetch(r);
         row.pairs(raw_d, d); row.pairs(raw_u, u); row.pairs(raw_x, x); row.pairs(raw_q, q);
-        if constexpr(GATE) row.pairs(raw_gate, gate);
         if(AHEAD && r + 1 < last) fetch(r + 1);
         // the statistics of both norms with the same barriers: means about the first elements, then squares
         if(layer){
@@ -426,24 +447,25 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 3 : TPR == 
                     }
                     add_to(K::SUM_GATE, i, d[2 * i], v0, d[2 * i + 1], v1);
                 }
-                const bool ends = r + 1 == sum_end;
+                const bool ends = r + 1 == group_end;
                 if(ends || r + 1 == last){
                     // the gate row's sum is complete here, or a piece of it: the group's rows go on with the next worker, or began with one before
                     float sum[E];
                     hand_out(K::SUM_GATE, sum);
-                    if(ends && sum_begin >= first) row.store(a.d_gate, sum_group * a.lddg, sum);
-                    else{
-                        float* piece = a.pieces + ((long long)worker * 2 + (sum_begin >= first ? 1 : 0)) * a.dim;
-#pragma unroll
-                        for(int e = 0; e < E; e++) if(row.inside(e)) piece[row.column(e / VEC) + e % VEC] = sum[e];
-                    }
+                    if(ends && group_begin >= first) row.store(a.d_gate, group * a.lddg, sum);
+                    else row.store_sums(a.pieces + ((long long)worker * 2 + (group_begin >= first ? 1 : 0)) * a.dim, sum);
 #pragma unroll
                     for(int i = 0; i < E / 4; i++) kept.at(K::SUM_GATE, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    sum_group++; sum_begin = sum_end; sum_end = min((long long)a.rows, sum_end + a.gate_rows);
                 }
             }
 #pragma unroll
-            for(int i = 0; i < P; i++) d[i] = mul2(d[i], gate[i]);
+            for(int i = 0; i < P; i++) d[i] = mul2(d[i], make_float2(to_float(raw_gate.e[2 * i]), to_float(raw_gate.e[2 * i + 1])));
+            if(r + 1 == group_end && r + 1 < last){
+                group++;
+                group_begin = group_end;
+                group_end = min((long long)a.rows, group_end + a.gate_rows);
+                row.fetch(a.gate, group * a.ldg, raw_gate);
+            }
         }
         if(post){
             float2 gg = both(0.0f), gh = gg;
@@ -471,9 +493,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 3 : TPR == 
         if(a.d_params[i] && (BIAS || i % 2 == 0)){
             float sum[E];
             hand_out(sums[i], sum);
-            float* partial = a.partials + ((long long)i * a.workers + worker) * a.dim;
-#pragma unroll
-            for(int e = 0; e < E; e++) if(row.inside(e)) partial[row.column(e / VEC) + e % VEC] = sum[e];
+            row.store_sums(a.partials + ((long long)i * a.workers + worker) * a.dim, sum);
         }
 }
 
@@ -485,38 +505,38 @@ __device__ __forceinline__ GatePieces gate_pieces(const NormBackward& a, long lo
     return {group, w, (int)((end - 1) / a.rows_per_worker) - w + 1};
 }
 
-// The sums over the workers, in their order: blockIdx.y < SUMS the parameter gradients, behind them gate rows (few, of many pieces). 32 columns a CTA, 32 threads a column.
+// The sums over the workers, in their order: blockIdx.y < n_sums the parameter gradients, behind them gate rows (few, of many pieces). 32 columns a CTA, 16 threads a column.
 template <typename T>
-__global__ void __launch_bounds__(1024) norm_backward_sums_kernel(NormBackward a){
-    __shared__ float shared[32][33];
+__global__ void __launch_bounds__(512) norm_backward_sums_kernel(NormBackward a){
+    __shared__ float shared[16][33];
     after_predecessor();
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    const bool parameter = blockIdx.y < SUMS;
+    const bool parameter = (int)blockIdx.y < a.n_sums;
+    const int index = parameter ? a.sums[blockIdx.y] : 0;
     const float* part; long long stride; int n, skip = 0;
     GatePieces g{};
-    if(parameter){
-        if(!a.d_params[blockIdx.y]) return;
-        part = a.partials + (long long)blockIdx.y * a.workers * a.dim; stride = a.dim; n = a.workers;
-    }
+    if(parameter){ part = a.partials + (long long)index * a.workers * a.dim; stride = a.dim; n = a.workers; }
     else{
-        g = gate_pieces(a, blockIdx.y - SUMS);
+        g = gate_pieces(a, blockIdx.y - a.n_sums);
         if(g.n == 1) return;
         part = a.pieces + 2ll * g.first * a.dim; stride = 2ll * a.dim; n = g.n; skip = a.dim;
     }
     float v = 0.0f;
     if(c < a.dim)
-#pragma unroll 4
-        for(int i = slice; i < n; i += 32) v += part[i * stride + (i == 0 ? skip : 0) + c];
+        for(int i = slice; i < n; i += 128){                 // eight loads under way
+            float e[8];
+#pragma unroll
+            for(int j = 0; j < 8; j++) e[j] = i + 16 * j < n ? part[(i + 16 * j) * stride + (i + 16 * j == 0 ? skip : 0) + c] : 0.0f;
+#pragma unroll
+            for(int j = 0; j < 8; j++) v += e[j];
+        }
     shared[slice][lane] = v;
     __syncthreads();
-    // a warp a column: its 32 slices, summed in a fixed tree
-    v = shared[lane][slice];
+    if(slice || c >= a.dim) return;
 #pragma unroll
-    for(int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    const int column = blockIdx.x * 32 + slice;
-    if(lane || column >= a.dim) return;
-    if(parameter) a.d_params[blockIdx.y][column] = a.accumulate ? a.d_params[blockIdx.y][column] + v : v;
-    else static_cast<T*>(a.d_gate)[g.group * a.lddg + column] = from_float<T>(v);
+    for(int i = 1; i < 16; i++) v += shared[i][lane];
+    if(parameter){ float* out = a.d_params[index] + c; *out = a.accumulate ? *out + v : v; }
+    else static_cast<T*>(a.d_gate)[g.group * a.lddg + c] = from_float<T>(v);
 }
 // The same for many gate rows of few pieces: blockIdx.y is the worker behind a boundary, a thread a column.
 template <typename T>
@@ -531,25 +551,12 @@ __global__ void __launch_bounds__(256) norm_backward_gates_kernel(NormBackward a
     static_cast<T*>(a.d_gate)[g.group * a.lddg + c] = from_float<T>(v);
 }
 
-template <int TPR, int E> struct Shape { static constexpr int tpr = TPR, e = E; };
-// Threads and elements per thread that hold a row: 16 elements a thread, 8 of fp32, so that the raw row that is under way takes the same registers either way
-template <typename T, typename F>
-static int dispatch_row(int dim, F f){
-    constexpr int E = sizeof(T) == 4 ? 8 : 16;
-    if(dim <= 32 * E) return f(Shape<32, E>{});
-    if(dim <= 128 * E) return f(Shape<128, E>{});
-    if(dim <= 256 * E) return f(Shape<256, E>{});
-    if constexpr(E == 8) if(dim > 512 * E) return f(Shape<1024, E>{});
-    return f(Shape<512, E>{});
-}
-
-// Workers of the backward pass and the consecutive rows that each takes: what is resident at once (rows of up to 512 elements: 12 workers a multiprocessor, and so on), a row
-// each where there are fewer rows than that, then four, so that the sums over the workers stay small against the rows.
+// Workers of the backward pass, and the consecutive rows that each takes: as many as are resident at once, a row each where there are fewer rows than that.
+template <typename T>
 static void plan_workers(int rows, int dim, int* workers, int* rows_per_worker){
-    const int most = NUM_SMS * (dim <= 512 ? 12 : dim <= 2048 ? 4 : dim <= 4096 ? 2 : 1);
-    const int per = rows <= 4 * most ? (rows <= most ? 1 : 4) : (rows - 1) / most + 1;
-    *rows_per_worker = per;
-    *workers = (rows - 1) / per + 1;
+    const int most = dispatch_row<T>(dim, [](auto shape){ return NUM_SMS * backward_ctas<T>(decltype(shape)::tpr, decltype(shape)::e) * (decltype(shape)::tpr == 32 ? 4 : 1); });
+    *rows_per_worker = (rows - 1) / most + 1;
+    *workers = (rows - 1) / *rows_per_worker + 1;
 }
 
 template <typename T, int VEC, int TPR, int E>
@@ -622,9 +629,10 @@ int b200rl_norm_residual_forward(int type, int post, const float* post_weight, c
 
 size_t b200rl_norm_residual_backward_scratch_bytes(int rows, int dim){
     if(rows < 1 || dim < 1 || dim > B200RL_NORM_MAX_DIM) return 0;
-    int workers, per;
-    plan_workers(rows, dim, &workers, &per);
-    return (size_t)workers * (SUMS + 2) * dim * sizeof(float);
+    int workers, workers32, per;
+    plan_workers<__half>(rows, dim, &workers, &per);
+    plan_workers<float>(rows, dim, &workers32, &per);
+    return (size_t)(workers > workers32 ? workers : workers32) * (SUMS + 2) * dim * sizeof(float);
 }
 
 int b200rl_norm_residual_backward(int type, int post, const float* post_weight, const float* post_bias, const void* branch, int ldb, const void* gate, int ldg,
@@ -654,7 +662,7 @@ int b200rl_norm_residual_backward(int type, int post, const float* post_weight, 
     NormBackward a{branch, row_pitch(ldb, rows, dim), gate, row_pitch(ldg, gates, dim), gate_rows, out, row_pitch(ldo, rows, dim), d_out, row_pitch(lddo, rows, dim),
                    d_normed, row_pitch(lddn, rows, dim), d_branch, row_pitch(lddb, rows, dim), d_residual, row_pitch(lddr, rows, dim), d_gate, row_pitch(lddg, gates, dim),
                    post_weight, post_bias, pre_weight, {d_post_weight, d_post_bias, d_pre_weight, d_pre_bias}};
-    plan_workers(rows, dim, &a.workers, &a.rows_per_worker);
+    if(type == B200RL_TYPE_FLOAT32) plan_workers<float>(rows, dim, &a.workers, &a.rows_per_worker); else plan_workers<__half>(rows, dim, &a.workers, &a.rows_per_worker);
     a.partials = static_cast<float*>(scratch);
     a.pieces = a.partials + (size_t)SUMS * a.workers * dim;
     a.post = post; a.pre = pre; a.rows = rows; a.dim = dim; a.accumulate = accumulate; a.scale = scale; a.epsilon = epsilon;
@@ -662,6 +670,7 @@ int b200rl_norm_residual_backward(int type, int post, const float* post_weight, 
     const bool vector = dim % n == 0 && (!branch || rows_aligned(branch, a.ldb, e)) && (!gate || rows_aligned(gate, a.ldg, e)) && (pre == B200RL_NORM_NONE || rows_aligned(out, a.ldo, e)) &&
                         (!d_out || rows_aligned(d_out, a.lddo, e)) && (!d_normed || rows_aligned(d_normed, a.lddn, e)) && (!d_branch || rows_aligned(d_branch, a.lddb, e)) &&
                         (!d_residual || rows_aligned(d_residual, a.lddr, e)) && (!d_gate || rows_aligned(d_gate, a.lddg, e));
+    for(int i = 0; i < SUMS; i++) if(a.d_params[i]) a.sums[a.n_sums++] = i;
     const bool bias = d_post_bias || d_pre_bias || (post_bias && gate);
     int rc = B200RL_ERR_UNSUPPORTED;
     B200RL_DISPATCH_TYPE(type, rc = dispatch_row<T>(dim, [&](auto shape){
@@ -673,9 +682,9 @@ int b200rl_norm_residual_backward(int type, int post, const float* post_weight, 
     }))
     if(rc) return rc;
     const bool shared_gates = d_gate && a.workers > 1 && gate_rows > 1, few_gates = shared_gates && gates <= 32;
-    if(few_gates || d_post_weight || d_post_bias || d_pre_weight || d_pre_bias){
-        const dim3 grid((dim + 31) / 32, SUMS + (few_gates ? gates : 0));
-        B200RL_DISPATCH_TYPE(type, B200RL_CUDA_TRY(launch_after(norm_backward_sums_kernel<T>, grid, dim3(1024), 0, (cudaStream_t)stream, a)))
+    if(few_gates || a.n_sums){
+        const dim3 grid((dim + 31) / 32, a.n_sums + (few_gates ? gates : 0));
+        B200RL_DISPATCH_TYPE(type, B200RL_CUDA_TRY(launch_after(norm_backward_sums_kernel<T>, grid, dim3(512), 0, (cudaStream_t)stream, a)))
     }
     if(shared_gates && !few_gates){
         const dim3 grid((dim + 255) / 256, a.workers - 1);
