@@ -16,39 +16,56 @@ struct Dropout {
     uint32_t stream_id;
 };
 
-// A thread takes the eight elements of a block. VECTOR: they lie in one row, 16-byte accesses.
-template <typename T, bool VECTOR>
+// How the elements lie: FLAT: one after another from the first row to the last in every operand, ROWS: the eight elements of a block lie in one row, both by 16-byte
+// accesses; ANY: one by one.
+enum { FLAT, ROWS, ANY };
+
+// the four words of block b: a draw of 16 bits for each of its elements
+__device__ __forceinline__ void draw_block(const Dropout& d, unsigned long long call, unsigned long long b, uint32_t (&c)[4]){
+    c[0] = (uint32_t)b; c[1] = (uint32_t)call; c[2] = (uint32_t)(call >> 32); c[3] = 0x80000000u + ((uint32_t)(b >> 32) << 16) + d.stream_id;
+    Philox::block(c, (uint32_t)d.seed, (uint32_t)(d.seed >> 32));
+}
+__device__ __forceinline__ float drop(const Dropout& d, const uint32_t (&c)[4], int e, float v){
+    return ((c[e >> 1] >> (16 * (e & 1))) & 0xFFFFu) >= d.threshold ? v * d.scale : 0.0f;
+}
+
+// A thread takes the eight elements of a block. Bound by memory: 16384 x 4096 bfloat16 with a residual moves 6 bytes an element; the ten rounds of a block cost its eight elements about ten instructions each, half of what the loads leave room for -- 32 bits an element would take all of it.
+template <typename T, int LAYOUT>
 __global__ void __launch_bounds__(256) dropout_kernel(Dropout d){
-    const unsigned long long n = (unsigned long long)d.rows * d.cols, blocks = (n + 7) / 8, call = d.call + (d.call_counter ? *d.call_counter : 0ull);
+    after_predecessor();
+    const unsigned long long n = (unsigned long long)d.rows * d.cols, blocks = (n + 7) / 8, call = d.call + (d.call_counter ? *opaque(d.call_counter) : 0ull);
+    const T *x = static_cast<const T*>(d.x), *residual = static_cast<const T*>(d.residual);
+    T* y = static_cast<T*>(d.y);
     for(unsigned long long b = blockIdx.x * 256ull + threadIdx.x; b < blocks; b += gridDim.x * 256ull){
-        uint32_t c[4] = {(uint32_t)b, (uint32_t)call, (uint32_t)(call >> 32), 0x80000000u + ((uint32_t)(b >> 32) << 16) + d.stream_id};
-        Philox::block(c, (uint32_t)d.seed, (uint32_t)(d.seed >> 32));
-        long long row = (long long)(b * 8 / d.cols); int col = (int)(b * 8 - (unsigned long long)row * d.cols);
-        if constexpr(VECTOR){
-            constexpr int N = 16 / sizeof(T);
+        uint32_t c[4];
+        long long row = 0, col = (long long)(b * 8);
+        if constexpr(LAYOUT != FLAT){ row = (long long)(b * 8 / d.cols); col = (long long)(b * 8) - row * d.cols; }
+        if(LAYOUT != ANY && b * 8 + 8 <= n){
+            constexpr int N = 16 / sizeof(T), PARTS = 8 / N;
+            float v[PARTS][N], r[PARTS][N];
 #pragma unroll
-            for(int part = 0; part < 8 / N; part++){
-                float v[N], r[N];
-                load_elements(static_cast<const T*>(d.x) + row * d.ldx + col + part * N, v);
-                if(d.residual) load_elements(static_cast<const T*>(d.residual) + row * d.ldr + col + part * N, r);
+            for(int part = 0; part < PARTS; part++){
+                load_elements(x + row * d.ldx + col + part * N, v[part]);
+                if(residual) load_elements(residual + row * d.ldr + col + part * N, r[part]);
+            }
+            draw_block(d, call, b, c);
 #pragma unroll
-                for(int i = 0; i < N; i++){
-                    const int e = part * N + i;
-                    const uint32_t draw = (c[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                    v[i] = (draw >= d.threshold ? v[i] * d.scale : 0.0f) + (d.residual ? r[i] : 0.0f);
-                }
-                store_elements(static_cast<T*>(d.y) + row * d.ldy + col + part * N, v);
+            for(int part = 0; part < PARTS; part++){
+#pragma unroll
+                for(int i = 0; i < N; i++) v[part][i] = drop(d, c, part * N + i, v[part][i]) + (residual ? r[part][i] : 0.0f);
+                store_elements(y + row * d.ldy + col + part * N, v[part]);
             }
         }
         else{
+            draw_block(d, call, b, c);
 #pragma unroll
             for(int e = 0; e < 8; e++){
                 if(b * 8 + e < n){
-                    const uint32_t draw = (c[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                    float v = draw >= d.threshold ? to_float(static_cast<const T*>(d.x)[row * d.ldx + col]) * d.scale : 0.0f;
-                    if(d.residual) v += to_float(static_cast<const T*>(d.residual)[row * d.ldr + col]);
-                    static_cast<T*>(d.y)[row * d.ldy + col] = from_float<T>(v);
-                    if(++col == d.cols){ col = 0; row++; }
+                    float v = drop(d, c, e, to_float(x[row * d.ldx + col]));
+                    if(residual) v += to_float(residual[row * d.ldr + col]);
+                    y[row * d.ldy + col] = from_float<T>(v);
+                    col++;
+                    if constexpr(LAYOUT != FLAT) if(col == d.cols){ col = 0; row++; }
                 }
             }
         }
@@ -70,10 +87,11 @@ extern "C" int b200rl_dropout(int type, const void* x, int ldx, const void* resi
     d.threshold = (uint32_t)((double)p * 65536.0 + 0.5);
     d.scale = d.threshold < 65536u ? 65536.0f / (float)(65536u - d.threshold) : 0.0f;
     d.seed = seed; d.call = call_index; d.call_counter = call_counter; d.stream_id = stream_id;
+    const bool flat = d.ldx == cols && d.ldy == cols && (!residual || d.ldr == cols) && rows_aligned(x, 16, e) && rows_aligned(y, 16, e) && (!residual || rows_aligned(residual, 16, e));
     const bool vector = cols % 8 == 0 && rows_aligned(x, d.ldx, e) && rows_aligned(y, d.ldy, e) && (!residual || rows_aligned(residual, d.ldr, e));
     const unsigned long long blocks = ((unsigned long long)rows * cols + 7) / 8, ctas = (blocks + 255) / 256;
-    const unsigned grid = (unsigned)(ctas < NUM_SMS * 8 ? ctas : NUM_SMS * 8);
-    B200RL_DISPATCH_TYPE(type, if(vector) dropout_kernel<T, true><<<grid, 256, 0, (cudaStream_t)stream>>>(d); else dropout_kernel<T, false><<<grid, 256, 0, (cudaStream_t)stream>>>(d))
-    B200RL_LAUNCH_CHECK("dropout");
+    const dim3 grid((unsigned)(ctas < NUM_SMS * 8 ? ctas : NUM_SMS * 8));
+    B200RL_DISPATCH_TYPE(type, B200RL_CUDA_TRY(launch_after(flat ? dropout_kernel<T, FLAT> : vector ? dropout_kernel<T, ROWS> : dropout_kernel<T, ANY>, grid, dim3(256), 0,
+                                                            (cudaStream_t)stream, d)))
     return B200RL_OK;
 }

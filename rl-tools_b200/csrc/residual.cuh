@@ -47,15 +47,26 @@ template <typename T, int N> __device__ __forceinline__ void store_elements(T* p
     }
 }
 
-// activation and its slope, the framework's definitions and two more
+// Activations and their slopes: the framework's definitions and two more, with few instructions, since they run on every element that a product leaves (a tile of 128 x 256 over
+// 1024 k takes the tensor core 8,200 cycles; 256 threads that spend 45 instructions an element on erff take 11,500). Errors stay below 1e-6, a thousandth of the rounding to 16 bits.
+//   Phi(x): erfc by Abramowitz and Stegun, "Handbook of Mathematical Functions", 7.1.26: erfc(z) = t (a1 + t (a2 + ...)) exp(-z^2) within 1.5e-7, t = 1 / (1 + p z), z >= 0
+struct NormalTail { float phi, density; };                               // Phi(x) and exp(-x^2 / 2)
+__device__ __forceinline__ NormalTail normal_tail(float x){
+    const float z = fabsf(x) * 0.70710678118654752f, t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f)), density = __expf(-0.5f * x * x);
+    const float tail = 0.5f * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * density;
+    return {x < 0.0f ? tail : 1.0f - tail, density};
+}
+__device__ __forceinline__ float fast_sigmoid(float x){ return __fdividef(1.0f, 1.0f + __expf(-x)); }      // exp(-x) = inf: 1 / inf = 0
 template <int ACT> __device__ __forceinline__ float residual_activation(float x){
-    if constexpr(ACT == B200RL_ACT_GELU) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
-    else if constexpr(ACT == B200RL_ACT_SILU) return x / (1.0f + expf(-x));
+    if constexpr(ACT == B200RL_ACT_GELU) return x * normal_tail(x).phi;
+    else if constexpr(ACT == B200RL_ACT_SILU) return x * fast_sigmoid(x);
+    else if constexpr(ACT == B200RL_ACT_SIGMOID) return fast_sigmoid(x);
     else return activation<ACT>(x);
 }
 template <int ACT> __device__ __forceinline__ float residual_d_activation(float x){
-    if constexpr(ACT == B200RL_ACT_GELU) return 0.5f * (1.0f + erff(x * 0.70710678118654752f)) + x * (0.39894228040143268f * expf(-0.5f * x * x));
-    else if constexpr(ACT == B200RL_ACT_SILU){ const float s = 1.0f / (1.0f + expf(-x)); return s * (1.0f + x * (1.0f - s)); }
+    if constexpr(ACT == B200RL_ACT_GELU){ const NormalTail n = normal_tail(x); return fmaf(x * 0.39894228040143268f, n.density, n.phi); }
+    else if constexpr(ACT == B200RL_ACT_SILU){ const float s = fast_sigmoid(x); return s * fmaf(x, 1.0f - s, 1.0f); }
+    else if constexpr(ACT == B200RL_ACT_SIGMOID){ const float s = fast_sigmoid(x); return s * (1.0f - s); }
     else return d_activation<ACT>(x);
 }
 #define B200RL_DISPATCH_RESIDUAL_ACT(act, ...) \
