@@ -174,26 +174,6 @@ struct Row {
     }
 };
 
-// Pairs of fp32 values: one instruction for both.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c){
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)), "l"(reinterpret_cast<const unsigned long long&>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b){
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b){
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
-    return d;
-}
-__device__ __forceinline__ float2 both(float v){ return make_float2(v, v); }
-__device__ __forceinline__ float across(float2 v){ return v.x + v.y; }
-
 // v <- (v - mean) rstd in place (0 behind the row's end); returns rstd. The mean is summed about the row's first element: a constant row has variance 0 whatever its value,
 // and the error of the mean goes by the row's spread.
 template <int TPR, typename R, int P>

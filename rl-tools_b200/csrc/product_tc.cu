@@ -4,7 +4,8 @@
 //
 // A CTA (or a pair of CTAs: CG = 2, one MMA over both SMs, each holding half of A and half of B) is persistent over output tiles of 128 CG x BN. Its warps:
 //   0  loads: stages of 64 k through a ring          1  issues the MMAs          2, 3  row sums of A (the bias gradient), straight from its matrix, beside the products
-//   4-11  epilogue: 32 rows x BN / 2 columns each, from one of two accumulators while the tensor core fills the other
+//   4-19  epilogue: 32 rows x BN / 4 columns each, from one of two accumulators while the tensor core fills the other. Sixteen warps, because a warp's way from tensor memory to the
+//         outputs is a chain of waits: with eight, the epilogue of a tile (10,000 cycles) was longer than its products over 1024 k (8,200)
 // Weight gradients and partial sums (EPI_SUM) are summed in pieces of PIECE k: the tensor core's accumulator truncates with every addition, which over a long batch adds up
 // (4,096 additions lose 1e-4); pieces of 32 additions are added in registers with rounding, while the next piece runs.
 #include "product.cuh"
@@ -17,9 +18,9 @@ namespace b200rl {
 namespace {
 constexpr int KB = 64;                                   // k of a stage: 128 bytes
 constexpr int PIECE = 512;                               // k in one accumulator of EPI_SUM
-constexpr int EPI_WARPS = 8, EPI_THREADS = EPI_WARPS * 32, THREADS = 128 + EPI_THREADS;
+constexpr int EPI_WARPS = 16, EPI_THREADS = EPI_WARPS * 32, THREADS = 128 + EPI_THREADS;
 constexpr uint32_t A_BYTES = 128 * 128;
-constexpr uint32_t STAGING = 8192;                       // per epilogue warp: two slabs of 32 rows x up to 128 bytes
+constexpr uint32_t STAGING = 4096;                       // per epilogue warp: a slab of 32 x 32 fp32
 constexpr uint32_t SMEM_LIMIT = 232448;
 constexpr long long WAIT_LIMIT = 2000000000LL;           // cycles: about a second
 constexpr int SUM_COLUMNS = 16, SUM_THREADS = 64;        // columns of a work item of the row sums: 32 bytes, a sector
@@ -38,10 +39,10 @@ struct TcArgs {
     const float* bias;
     const void* add; long long ld_add;
     void* pre; long long ld_pre;
-    void* out; long long ld_out;
+    void* out; long long ld_out, split_stride;           // of EPI_SUM: elements from one split's sums to the next
     float scale;
     int act, accumulate;
-    int fast;                                            // 16-bit outputs by TMA, 16-byte loads of add and pre
+    int fast;                                            // rows of the outputs, add and pre start on 16-byte boundaries
     const void* sum_source; long long ld_sum; float* sums; // row sums of A: [splits][m] (or the gradient itself: one split)
     int sums_accumulate;
 };
@@ -65,15 +66,6 @@ template <int CG> __device__ __forceinline__ void load_box(void* smem, const CUt
                      :: "r"(tc::smem_u32(smem)), "l"(map), "r"(leader_address(bar)), "r"(x), "r"(y) : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map){ asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory"); }
-__device__ __forceinline__ void store_box_2d(const CUtensorMap* map, const void* smem, int x, int y){
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" :: "l"(map), "r"(tc::smem_u32(smem)), "r"(x), "r"(y) : "memory");
-}
-__device__ __forceinline__ void store_box_3d(const CUtensorMap* map, const void* smem, int x, int y, int z){
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" :: "l"(map), "r"(tc::smem_u32(smem)), "r"(x), "r"(y), "r"(z) : "memory");
-}
-__device__ __forceinline__ void add_box_3d(const CUtensorMap* map, const void* smem, int x, int y, int z){
-    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" :: "l"(map), "r"(tc::smem_u32(smem)), "r"(x), "r"(y), "r"(z) : "memory");
-}
 template <int CG> __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate){
     if constexpr(CG == 1) tc::mma_f16_ss(d, a, b, idesc, accumulate);
     else asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
@@ -120,87 +112,150 @@ template <typename T> __device__ __forceinline__ float2 unpack(uint32_t v);
 template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t v){ return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t v){ return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
-// 8 N consecutive elements of a row whose start is 16-byte aligned; elements from `end` on are 0
-template <typename T, int N> __device__ __forceinline__ void load_slab_row(uint4 (&raw)[N], const T* row, int col, int end, bool there){
-#pragma unroll
-    for(int i = 0; i < N; i++){
-        raw[i] = make_uint4(0, 0, 0, 0);
-        const int c = col + 8 * i;
-        if(!there || c >= end) continue;
-        if(c + 8 <= end) raw[i] = *reinterpret_cast<const uint4*>(row + c);
-        else{
-            union { uint4 v; T e[8]; } u;
-            u.v = raw[i];
-#pragma unroll
-            for(int j = 0; j < 8; j++) if(c + j < end) u.e[j] = row[c + j];
-            raw[i] = u.v;
-        }
-    }
-}
-// a row of a slab of 32 rows x W 16-bit elements, as the tensor maps of the outputs have it: rows of 64 bytes with the 64-byte swizzle or of 128 with the 128-byte one
-template <typename T, int W> __device__ __forceinline__ void store_slab_row(uint8_t* slab, int lane, const float (&v)[W]){
-#pragma unroll
-    for(int c = 0; c < W / 8; c++){
-        uint4 q = make_uint4(pack<T>(v[8 * c], v[8 * c + 1]), pack<T>(v[8 * c + 2], v[8 * c + 3]), pack<T>(v[8 * c + 4], v[8 * c + 5]), pack<T>(v[8 * c + 6], v[8 * c + 7]));
-        *reinterpret_cast<uint4*>(slab + lane * (2 * W) + ((c ^ (W == 64 ? lane & 7 : (lane >> 1) & 3)) << 4)) = q;
-    }
-}
-template <typename T, int N> __device__ __forceinline__ void unpack_chunk(float (&f)[8], const uint4 (&raw)[N], int i){
-    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+template <typename T> __device__ __forceinline__ void unpack_chunk(float (&f)[8], const uint4& raw){
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for(int e = 0; e < 4; e++){ const float2 p = unpack<T>(u[e]); f[2 * e] = p.x; f[2 * e + 1] = p.y; }
 }
-template <int ACT, int W> __device__ __forceinline__ void activate(float (&v)[W]){
+template <typename T> __device__ __forceinline__ uint4 pack_chunk(const float (&v)[8]){ return make_uint4(pack<T>(v[0], v[1]), pack<T>(v[2], v[3]), pack<T>(v[4], v[5]), pack<T>(v[6], v[7])); }
+// eight consecutive elements at p (16-byte aligned), of which `count` exist
+template <typename T> __device__ __forceinline__ uint4 load_chunk(const T* p, int count){
+    if(count >= 8) return *reinterpret_cast<const uint4*>(p);
+    union { uint4 v; T e[8]; } u;
+    u.v = make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for(int c = 0; c < W; c++) v[c] = residual_activation<ACT>(v[c]);
+    for(int j = 0; j < 8; j++) if(j < count) u.e[j] = p[j];
+    return u.v;
 }
-template <int ACT, typename T, int W> __device__ __forceinline__ void times_slope(float (&v)[W], const uint4 (&pre)[W / 8]){
+template <typename T> __device__ __forceinline__ void store_chunk(T* p, const uint4& v, int count){
+    if(count >= 8) *reinterpret_cast<uint4*>(p) = v;
+    else{
+        union { uint4 v; T e[8]; } u;
+        u.v = v;
 #pragma unroll
-    for(int i = 0; i < W / 8; i++){
-        float p[8];
-        unpack_chunk<T>(p, pre, i);
-#pragma unroll
-        for(int c = 0; c < 8; c++) v[8 * i + c] *= residual_d_activation<ACT>(p[c]);
+        for(int j = 0; j < 8; j++) if(j < count) p[j] = u.e[j];
     }
 }
 
-template <int N> __device__ __forceinline__ void load_bias(float (&bias)[N], const TcArgs& a, int col){
+// A slab: 32 x 32 sums, transposed through shared memory from a lane a row (as tensor memory is read) to accesses along rows of the matrices, so that every global access of the warp
+// covers whole sectors. 16-byte piece c of row r lies at piece c ^ (r % 8): neither direction has bank conflicts. Measured against outputs by TMA: those wait in the TMA unit's queue
+// behind up to five stages of operand loads, 2,500 cycles a slab, and a warp has no third buffer (16384 x 4096 x 4096 with a residual 470 us).
+__device__ __forceinline__ void slab_in(uint8_t* slab, const uint32_t (&r)[32], int lane){
 #pragma unroll
-    for(int h = 0; h < N; h++) bias[h] = a.bias && col + 32 * h < a.n ? a.bias[col + 32 * h] : 0.0f;
+    for(int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(slab + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
 }
+__device__ __forceinline__ float4 slab_out(const uint8_t* slab, int row, int piece){ return *reinterpret_cast<const float4*>(slab + row * 128 + ((piece ^ (row & 7)) << 4)); }
+__device__ __forceinline__ float slab_element(const uint8_t* slab, int row, int column){ return *reinterpret_cast<const float*>(slab + row * 128 + (((column >> 2) ^ (row & 7)) << 4) + (column & 3) * 4); }
 
-// One 32 x 32 slab whose operands or outputs have rows at odd addresses: transposed through shared memory, so that a lane has a column and every access of the warp goes
-// along a row.
-template <typename T, int EPI>
-__device__ __forceinline__ void finish_slab_by_rows(const TcArgs& a, float* buffer, const float* v, int row0, int col, int lane){
+// The operands of a slab's epilogue that lie in memory, 16-bit rows on 16-byte boundaries: a lane has eight columns of every eighth row. WHOLE: all of the slab is inside the matrix.
+struct SlabOperands { uint4 add[4], pre[4]; };
+template <typename T> __device__ __forceinline__ void fetch_chunks(uint4 (&raw)[4], const T* p, long long ld, int rows, int count){
+    if(rows >= 32 && count >= 8)
 #pragma unroll
-    for(int c = 0; c < 32; c++) buffer[lane * 33 + c] = v[c];
-    __syncwarp();
-    if(col < a.n){
-        const float bias = EPI == EPI_FORWARD && a.bias ? a.bias[col] : 0.0f;
+        for(int i = 0; i < 4; i++, p += 8 * ld) raw[i] = *reinterpret_cast<const uint4*>(p);
+    else
+#pragma unroll
+        for(int i = 0; i < 4; i++, p += 8 * ld) if(8 * i < rows && count > 0) raw[i] = load_chunk(p, count);
+}
+template <typename T, int EPI> __device__ __forceinline__ void fetch_slab(SlabOperands& o, const TcArgs& a, int row0, int col0, int lane){
+    const int col = col0 + 8 * (lane & 3), row = row0 + (lane >> 2), count = a.n - col, rows = row0 + 32 <= a.m ? 32 : a.m - row;
+    if(a.add) fetch_chunks(o.add, static_cast<const T*>(a.add) + (long long)row * a.ld_add + col, a.ld_add, rows, count);
+    if constexpr(EPI == EPI_INPUT) if(a.act != B200RL_ACT_IDENTITY) fetch_chunks(o.pre, static_cast<const T*>(a.pre) + (long long)row * a.ld_pre + col, a.ld_pre, rows, count);
+}
+template <typename T, int EPI, int ACT, bool WHOLE>
+__device__ __forceinline__ void finish_slab(const TcArgs& a, const uint8_t* slab, const SlabOperands& o, const float (&bias)[8], int row0, int col0, int lane){
+    const int col = col0 + 8 * (lane & 3), row = row0 + (lane >> 2), count = a.n - col, rows = a.m - row;
+    T* out = static_cast<T*>(a.out) + (long long)row * a.ld_out + col;
+    T* pre = EPI == EPI_FORWARD && a.pre ? static_cast<T*>(a.pre) + (long long)row * a.ld_pre + col : nullptr;
+#pragma unroll
+    for(int i = 0; i < 4; i++, out += 8 * a.ld_out){
+        const float4 lo = slab_out(slab, 8 * i + (lane >> 2), 2 * (lane & 3)), hi = slab_out(slab, 8 * i + (lane >> 2), 2 * (lane & 3) + 1);
+        float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}, add[8];
+        const bool there = WHOLE || (8 * i < rows && count > 0);
+        const int elements = WHOLE ? 8 : count;
+        if constexpr(EPI == EPI_FORWARD){
+            if(a.bias)
+#pragma unroll
+                for(int c = 0; c < 8; c++) v[c] += bias[c];
+            if(pre){
+                if(there) store_chunk(pre, pack_chunk<T>(v), elements);
+                pre += 8 * a.ld_pre;
+            }
+            activate8<ACT>(v);
+            if(a.add){
+                unpack_chunk<T>(add, o.add[i]);
+#pragma unroll
+                for(int c = 0; c < 8; c++) v[c] = fmaf(a.scale, v[c], add[c]);
+            }
+            else
+#pragma unroll
+                for(int c = 0; c < 8; c++) v[c] *= a.scale;
+        }
+        else{
+            if(a.add){
+                unpack_chunk<T>(add, o.add[i]);
+#pragma unroll
+                for(int c = 0; c < 8; c++) v[c] += add[c];
+            }
+            if constexpr(ACT != B200RL_ACT_IDENTITY){
+                unpack_chunk<T>(add, o.pre[i]);
+                times_slope8<ACT>(v, add);
+            }
+        }
+        if(there) store_chunk(out, pack_chunk<T>(v), elements);
+    }
+}
+// The same where rows start at odd addresses: a lane has a column
+template <typename T, int EPI>
+__device__ __forceinline__ void finish_slab_by_rows(const TcArgs& a, const uint8_t* slab, int row0, int col0, int lane){
+    const int col = col0 + lane;
+    if(col >= a.n) return;
+    const float bias = EPI == EPI_FORWARD && a.bias ? a.bias[col] : 0.0f;
+    const int rows = min(32, a.m - row0);
+#pragma unroll 4
+    for(int r = 0; r < rows; r++){
+        const long long row = row0 + r;
+        float x = slab_element(slab, r, lane);
+        const float add = a.add ? to_float(static_cast<const T*>(a.add)[row * a.ld_add + col]) : 0.0f;
+        if constexpr(EPI == EPI_FORWARD){
+            x += bias;
+            if(a.pre) static_cast<T*>(a.pre)[row * a.ld_pre + col] = from_float<T>(x);
+            B200RL_DISPATCH_RESIDUAL_ACT(a.act, x = residual_activation<ACT>(x))
+            x = fmaf(a.scale, x, add);
+        }
+        else{
+            x += add;
+            if(a.act != B200RL_ACT_IDENTITY){
+                const float p = to_float(static_cast<const T*>(a.pre)[row * a.ld_pre + col]);
+                B200RL_DISPATCH_RESIDUAL_ACT(a.act, x *= residual_d_activation<ACT>(p))
+            }
+        }
+        static_cast<T*>(a.out)[row * a.ld_out + col] = from_float<T>(x);
+    }
+}
+// A slab of an fp32 result
+__device__ __forceinline__ void store_sums(const TcArgs& a, const uint8_t* slab, int z, int row0, int col0, int lane){
+    float* out = static_cast<float*>(a.out) + z * a.split_stride;
+    if(a.fast && col0 + 32 <= a.n){
+#pragma unroll
+        for(int i = 0; i < 8; i++){
+            const int r = 4 * i + (lane >> 3);
+            if(row0 + r >= a.m) continue;
+            float4 v = slab_out(slab, r, lane & 7);
+            float4* p = reinterpret_cast<float4*>(out + (long long)(row0 + r) * a.ld_out + col0 + 4 * (lane & 7));
+            if(a.accumulate){ const float4 q = *p; v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w; }
+            *p = v;
+        }
+    }
+    else if(col0 + lane < a.n){
         const int rows = min(32, a.m - row0);
 #pragma unroll 4
         for(int r = 0; r < rows; r++){
-            const long long row = row0 + r;
-            float x = buffer[r * 33 + lane];
-            const float add = a.add ? to_float(static_cast<const T*>(a.add)[row * a.ld_add + col]) : 0.0f;
-            if constexpr(EPI == EPI_FORWARD){
-                x += bias;
-                if(a.pre) static_cast<T*>(a.pre)[row * a.ld_pre + col] = from_float<T>(x);
-                B200RL_DISPATCH_RESIDUAL_ACT(a.act, x = residual_activation<ACT>(x))
-                x = fmaf(a.scale, x, add);
-            }
-            else{
-                x += add;
-                if(a.act != B200RL_ACT_IDENTITY){
-                    const float p = to_float(static_cast<const T*>(a.pre)[row * a.ld_pre + col]);
-                    B200RL_DISPATCH_RESIDUAL_ACT(a.act, x *= residual_d_activation<ACT>(p))
-                }
-            }
-            static_cast<T*>(a.out)[row * a.ld_out + col] = from_float<T>(x);
+            float* p = out + (long long)(row0 + r) * a.ld_out + col0 + lane;
+            const float v = slab_element(slab, r, lane);
+            *p = a.accumulate ? *p + v : v;
         }
     }
-    __syncwarp();
 }
 
 template <typename T>
@@ -208,12 +263,11 @@ __device__ __forceinline__ void sum_rows(const TcArgs& a, float* shared, int tid
 
 template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI>
 __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_pre,
                                                                 const __grid_constant__ TcArgs a){
     constexpr int STAGES = stage_count(CG, BN);
     constexpr uint32_t STAGE = stage_bytes(CG, BN);
-    constexpr int CW = BN / 2, SW = CW < 64 ? CW : 64;                  // columns of an epilogue warp, of a slab of 16-bit outputs
-    static_assert(CW % SW == 0 && SW % 32 == 0);
+    constexpr int GROUPS = BN < 128 ? BN / 32 : 4, CW = BN / GROUPS, SLABS = CW / 32;       // groups of four epilogue warps at work; columns of a warp, slabs of them
+    static_assert(CW % 32 == 0);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* staging = base + STAGES * STAGE;
@@ -225,9 +279,9 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
     if(tid == 0){
-        prefetch_map(&map_a); prefetch_map(&map_b); prefetch_map(&map_out); prefetch_map(&map_pre);
+        prefetch_map(&map_a); prefetch_map(&map_b);
         for(int s = 0; s < STAGES; s++){ tc::mbar_init(full + s, 1); tc::mbar_init(empty + s, 1); }
-        for(int b = 0; b < 2; b++){ tc::mbar_init(acc_full + b, 1); tc::mbar_init(acc_empty + b, CG * EPI_WARPS); }
+        for(int b = 0; b < 2; b++){ tc::mbar_init(acc_full + b, 1); tc::mbar_init(acc_empty + b, CG * 4 * GROUPS); }
         tc::fence_mbar_init();
         *abort_flag = 0;
     }
@@ -242,7 +296,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     const int k_blocks = (a.k + KB - 1) / KB;
 
     if(warp < 4){
-        tc::setmaxnreg_dec<72>();
+        tc::setmaxnreg_dec<64>();
         if(warp == 0 && lane == 0){
             uint32_t it = 0;
             bool ok = true;
@@ -308,35 +362,36 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         __syncwarp();
     }
     else{
-        tc::setmaxnreg_inc<216>();
-        const int w = warp - 4, q = w & 3, half = w >> 2;                // tensor memory lanes 32 q .. +31, columns half CW .. +CW - 1
+        tc::setmaxnreg_inc<104>();
+        const int w = warp - 4, q = w & 3, group = w >> 2;               // tensor memory lanes 32 q .. +31, columns group CW .. +CW - 1
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
-        uint8_t* slabs = staging + w * STAGING;
-        uint32_t acc = 0, stored = 0;
+        uint8_t* slab = staging + w * STAGING;
+        uint32_t acc = 0;
         bool ok = true;
-        for(int t = first_tile; t < tiles && ok; t += tile_step){
+        for(int t = first_tile; t < tiles && ok && group < GROUPS; t += tile_step){
             const TileIndex i = tile_index(a, t);
-            const int row0 = i.m * 128 * CG + (int)rank * 128 + q * 32, col0 = i.n * BN + half * CW;
+            const int row0 = i.m * 128 * CG + (int)rank * 128 + q * 32, col0 = i.n * BN + group * CW;
             if constexpr(EPI == EPI_SUM){
                 const int kb_begin = i.z * a.split_blocks, kb_end = min(k_blocks, kb_begin + a.split_blocks);
                 const int pieces = (kb_end - kb_begin + PIECE / KB - 1) / (PIECE / KB);
-                float sum[CW / 32][32];
+                float sum[SLABS][32];
 #pragma unroll
-                for(int j = 0; j < CW / 32; j++)
+                for(int j = 0; j < SLABS; j++)
 #pragma unroll
                     for(int c = 0; c < 32; c++) sum[j][c] = 0.0f;
                 for(int p = 0; p < pieces; p++, acc++){
                     const uint32_t b = acc & 1;
                     if(!tc::mbar_wait_bounded(acc_full + b, (acc >> 1) & 1, WAIT_LIMIT)){ ok = false; break; }
                     tc::fence_after_thread_sync();
+                    constexpr int AT_ONCE = 1;                           // registers: 64 sums and 32 of these
 #pragma unroll
-                    for(int j = 0; j < CW / 32; j += SW / 32){
-                        uint32_t r[SW / 32][32];
+                    for(int j = 0; j < SLABS; j += AT_ONCE){
+                        uint32_t r[AT_ONCE][32];
 #pragma unroll
-                        for(int h = 0; h < SW / 32; h++) tc::tmem_ld_32x32(tmem + lanes + b * BN + half * CW + (j + h) * 32, r[h]);
+                        for(int h = 0; h < AT_ONCE; h++) tc::tmem_ld_32x32(tmem + lanes + b * BN + group * CW + (j + h) * 32, r[h]);
                         tc::tmem_wait_ld();
 #pragma unroll
-                        for(int h = 0; h < SW / 32; h++)
+                        for(int h = 0; h < AT_ONCE; h++)
 #pragma unroll
                             for(int c = 0; c < 32; c++) sum[j + h][c] += __uint_as_float(r[h][c]);
                     }
@@ -346,120 +401,48 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 }
                 if(!ok) break;
 #pragma unroll
-                for(int j = 0; j < CW / 32; j++){
-                    uint8_t* slab = slabs + (stored & 1) * 4096;
-                    if(lane == 0) tc::bulk_wait_read<1>();
-                    __syncwarp();
+                for(int j = 0; j < SLABS; j++){
+                    uint32_t r[32];
 #pragma unroll
-                    for(int c = 0; c < 8; c++)
-                        *reinterpret_cast<float4*>(slab + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(sum[j][4 * c], sum[j][4 * c + 1], sum[j][4 * c + 2], sum[j][4 * c + 3]);
-                    tc::fence_proxy_async_smem();
+                    for(int c = 0; c < 32; c++) r[c] = __float_as_uint(sum[j][c]);
                     __syncwarp();
-                    if(lane == 0){
-                        if(row0 < a.m && col0 + j * 32 < a.n){
-                            if(a.accumulate) add_box_3d(&map_out, slab, col0 + j * 32, row0, i.z);
-                            else store_box_3d(&map_out, slab, col0 + j * 32, row0, i.z);
-                        }
-                        tc::bulk_commit();
-                    }
-                    stored++;
+                    slab_in(slab, r, lane);
+                    __syncwarp();
+                    if(row0 < a.m && col0 + 32 * j < a.n) store_sums(a, slab, i.z, row0, col0 + 32 * j, lane);
                 }
             }
             else{
                 const uint32_t b = acc & 1, phase = (acc >> 1) & 1;
                 acc++;
-                const long long row = row0 + lane;
-                const bool there = row < a.m && a.fast;
-                const T* add_row = a.add ? static_cast<const T*>(a.add) + row * a.ld_add : nullptr;
-                const T* pre_row = EPI == EPI_INPUT && a.act != B200RL_ACT_IDENTITY ? static_cast<const T*>(a.pre) + row * a.ld_pre : nullptr;
-                uint4 add_raw[SW / 8], pre_raw[EPI == EPI_INPUT ? SW / 8 : 1];
-                float bias[SW / 32];                                     // of columns lane, lane + 32
-                load_slab_row(add_raw, add_row, col0, a.n, there && add_row);
-                if constexpr(EPI == EPI_INPUT) load_slab_row(pre_raw, pre_row, col0, a.n, there && pre_row);
-                else load_bias(bias, a, col0 + lane);
+                SlabOperands o;
+                if(a.fast) fetch_slab<T, EPI>(o, a, row0, col0, lane);
                 if(!tc::mbar_wait_bounded(acc_full + b, phase, WAIT_LIMIT)){ ok = false; break; }
                 tc::fence_after_thread_sync();
+                uint32_t r[32];
+                tc::tmem_ld_32x32(tmem + lanes + b * BN + group * CW, r);
 #pragma unroll 1
-                for(int j = 0; j < CW / SW; j++){
-                    const int col = col0 + j * SW;
-                    float v[SW];
-                    {
-                        uint32_t r[SW / 32][32];
-#pragma unroll
-                        for(int h = 0; h < SW / 32; h++) tc::tmem_ld_32x32(tmem + lanes + b * BN + half * CW + j * SW + h * 32, r[h]);
-                        tc::tmem_wait_ld();
-#pragma unroll
-                        for(int c = 0; c < SW; c++) v[c] = __uint_as_float(r[c / 32][c % 32]);
-                    }
-                    if(j == CW / SW - 1){
-                        tc::fence_before_thread_sync();
-                        __syncwarp();
-                        if(lane == 0) arrive_at_leader<CG>(acc_empty + b);
-                    }
+                for(int j = 0; j < SLABS; j++){
+                    const int col = col0 + j * 32;
+                    tc::tmem_wait_ld();
+                    __syncwarp();                                        // the slab before has been read
+                    slab_in(slab, r, lane);
+                    if(j + 1 < SLABS) tc::tmem_ld_32x32(tmem + lanes + b * BN + group * CW + (j + 1) * 32, r);
+                    else tc::fence_before_thread_sync();
+                    __syncwarp();
+                    if(j + 1 == SLABS && lane == 0) arrive_at_leader<CG>(acc_empty + b);
                     if(row0 >= a.m || col >= a.n) continue;
-                    if(!a.fast){
+                    if(!a.fast){ finish_slab_by_rows<T, EPI>(a, slab, row0, col, lane); continue; }
+                    float bias[8];
+                    if constexpr(EPI == EPI_FORWARD) if(a.bias)
 #pragma unroll
-                        for(int h = 0; h < SW / 32; h++) finish_slab_by_rows<T, EPI>(a, reinterpret_cast<float*>(slabs), v + 32 * h, row0, col + 32 * h + lane, lane);
-                        continue;
-                    }
-                    // two slabs in turn; with pre-activations to keep, one for each output
-                    const bool two = EPI == EPI_FORWARD && a.pre;
-                    uint8_t *slab = slabs + (two ? 0 : (stored & 1) * 4096), *pre_slab = slabs + 4096;
-                    if(lane == 0){ if(two) tc::bulk_wait_read<0>(); else tc::bulk_wait_read<1>(); }
-                    __syncwarp();
-                    if constexpr(EPI == EPI_FORWARD){
-                        if(a.bias){                                      // a lane needs every column's: handed round through the slab
-                            float* all = reinterpret_cast<float*>(slab);
-#pragma unroll
-                            for(int h = 0; h < SW / 32; h++) all[h * 32 + lane] = bias[h];
-                            __syncwarp();
-#pragma unroll
-                            for(int c = 0; c < SW; c += 4){
-                                const float4 q = *reinterpret_cast<const float4*>(all + c);
-                                v[c] += q.x; v[c + 1] += q.y; v[c + 2] += q.z; v[c + 3] += q.w;
-                            }
-                            __syncwarp();
-                            if(j + 1 < CW / SW) load_bias(bias, a, col + SW + lane);
-                        }
-                        if(a.pre) store_slab_row<T, SW>(pre_slab, lane, v);
-                        B200RL_DISPATCH_RESIDUAL_ACT(a.act, activate<ACT>(v))
-#pragma unroll
-                        for(int i = 0; i < SW / 8; i++){
-                            float add[8];
-                            unpack_chunk<T>(add, add_raw, i);
-#pragma unroll
-                            for(int c = 0; c < 8; c++) v[8 * i + c] = fmaf(a.scale, v[8 * i + c], add[c]);
-                        }
-                        if(j + 1 < CW / SW) load_slab_row(add_raw, add_row, col + SW, a.n, there && add_row);
-                    }
-                    else{
-#pragma unroll
-                        for(int i = 0; i < SW / 8; i++){
-                            float add[8];
-                            unpack_chunk<T>(add, add_raw, i);
-#pragma unroll
-                            for(int c = 0; c < 8; c++) v[8 * i + c] += add[c];
-                        }
-                        if(j + 1 < CW / SW) load_slab_row(add_raw, add_row, col + SW, a.n, there && add_row);
-                        if(a.act != B200RL_ACT_IDENTITY){
-                            B200RL_DISPATCH_RESIDUAL_ACT(a.act, (times_slope<ACT, T, SW>(v, pre_raw)))
-                            if(j + 1 < CW / SW) load_slab_row(pre_raw, pre_row, col + SW, a.n, there && pre_row);
-                        }
-                    }
-                    store_slab_row<T, SW>(slab, lane, v);
-                    tc::fence_proxy_async_smem();
-                    __syncwarp();
-                    if(lane == 0){
-                        store_box_2d(&map_out, slab, col, row0);
-                        if(two) store_box_2d(&map_pre, pre_slab, col, row0);
-                        tc::bulk_commit();
-                    }
-                    stored++;
+                        for(int c = 0; c < 8; c++) bias[c] = a.bias[min(col + 8 * (lane & 3) + c, a.n - 1)];
+                    if(row0 + 32 <= a.m && col + 32 <= a.n){ B200RL_DISPATCH_RESIDUAL_ACT(a.act, (finish_slab<T, EPI, ACT, true>(a, slab, o, bias, row0, col, lane))) }
+                    else { B200RL_DISPATCH_RESIDUAL_ACT(a.act, (finish_slab<T, EPI, ACT, false>(a, slab, o, bias, row0, col, lane))) }
+                    if(j + 1 < SLABS) fetch_slab<T, EPI>(o, a, row0, col + 32, lane);
                 }
             }
         }
         if(!ok){ *abort_flag = 1; g_product_tc_error = 1; }
-        if(lane == 0) tc::bulk_wait_all<0>();
         __syncwarp();
     }
     tc::fence_before_thread_sync();
@@ -494,7 +477,7 @@ __device__ __forceinline__ void sum_rows(const TcArgs& a, float* shared, int tid
 #pragma unroll
                     for(int h = 0; h < 2; h++){
                         float e[8];
-                        unpack_chunk<T>(e, raw[i], h);
+                        unpack_chunk<T>(e, raw[i][h]);
 #pragma unroll
                         for(int c = 0; c < 8; c++) v[8 * h + c] += e[c];
                     }
@@ -608,18 +591,15 @@ static int encode_tiled(EncodeTiled* out){
     *out = f;
     return B200RL_OK;
 }
-// rows x cols with rows ld elements apart, boxes of box_rows x box_cols; planes > 1 (or three): a third dimension plane_stride elements apart
-static int make_map(CUtensorMap* map, CUtensorMapDataType type, int element, const void* p, long long rows, long long cols, long long ld, int box_rows, int box_cols, CUtensorMapSwizzle swizzle,
-                    bool three = false, long long planes = 1, long long plane_stride = 0){
+// an operand: rows x cols 16-bit elements with rows ld elements apart, boxes of box_rows x 64
+static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, long long rows, long long cols, long long ld, int box_rows){
     EncodeTiled encode;
     int rc = encode_tiled(&encode);
     if(rc) return rc;
-    // the pitch of a single row (or plane) is not used, but has to be a multiple of 16 bytes
-    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
-    const cuuint64_t pitch = rows > 1 ? (cuuint64_t)ld * element : ((cuuint64_t)cols * element + 15) / 16 * 16;
-    const cuuint64_t strides[2] = {pitch, planes > 1 ? (cuuint64_t)plane_stride * element : pitch * (cuuint64_t)rows};
-    const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, steps[3] = {1, 1, 1};
-    if(encode(map, type, three ? 3 : 2, const_cast<void*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    // the pitch of a single row is not used, but has to be a multiple of 16 bytes
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {rows > 1 ? (cuuint64_t)ld * 2 : ((cuuint64_t)cols * 2 + 15) / 16 * 16};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, steps[2] = {1, 1};
+    if(encode(map, type, 2, const_cast<void*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return B200RL_ERR_UNSUPPORTED;
     return B200RL_OK;
 }
@@ -653,7 +633,7 @@ static TcPlan plan_product(const Product& g, int epilogue){
     // operands that TMA cannot address are copied
     p.copy_a = !rows_aligned(g.a.p, g.a.ld, 2) && !(matrix_rows(g.a, g.m, g.k) <= 1 && reinterpret_cast<uintptr_t>(g.a.p) % 16 == 0);
     p.copy_b = !rows_aligned(g.b.p, g.b.ld, 2) && !(matrix_rows(g.b, g.n, g.k) <= 1 && reinterpret_cast<uintptr_t>(g.b.p) % 16 == 0);
-    p.partial = p.splits > 1 || (epilogue == EPI_SUM && g.out && !rows_aligned(g.out, g.ld_out, 4));
+    p.partial = p.splits > 1;
     p.ld_copy_a = (matrix_cols(g.a, g.m, g.k) + 7) / 8 * 8;
     p.ld_copy_b = (matrix_cols(g.b, g.n, g.k) + 7) / 8 * 8;
     p.ld_partial = (g.n + 31) / 32 * 32;
@@ -676,7 +656,7 @@ static int align_rows(const Operand& o, long long rows, long long cols, void* ds
 }
 
 template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI>
-static int launch_tc(const CUtensorMap (&maps)[4], const TcArgs& a, cudaStream_t s){
+static int launch_tc(const CUtensorMap (&maps)[2], const TcArgs& a, cudaStream_t s){
     auto* kernel = product_tc_kernel<CG, BN, A_ROWS, B_ROWS, T, EPI>;
     static std::atomic<int> groups[MAX_DEVICES];           // tiles that run at the same time: 0 until the kernel is set up on the device
     int dev = 0, sms = 0;
@@ -701,11 +681,11 @@ static int launch_tc(const CUtensorMap (&maps)[4], const TcArgs& a, cudaStream_t
     const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
     cfg.gridDim = (unsigned)(CG * (tiles < most ? tiles : most));
     cfg.numAttrs = 2;
-    B200RL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], a));
+    B200RL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], a));
     return B200RL_OK;
 }
 template <bool A_ROWS, bool B_ROWS, typename T, int EPI>
-static int launch_tile(const TcPlan& p, const CUtensorMap (&maps)[4], const TcArgs& a, cudaStream_t s){
+static int launch_tile(const TcPlan& p, const CUtensorMap (&maps)[2], const TcArgs& a, cudaStream_t s){
     if(p.cg == 2) return launch_tc<2, 256, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
     if(p.bn == 128) return launch_tc<1, 128, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
     return launch_tc<1, 64, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
@@ -740,17 +720,15 @@ static int product_tc_typed(const Product& g, int type, int epilogue, void* work
     a.idesc = 1u << 4 | format << 7 | format << 10 | (A.k_rows ? 1u << 15 : 0u) | (B.k_rows ? 1u << 16 : 0u) | (uint32_t)(p.bn / 8) << 17 | (uint32_t)(128 * p.cg / 16) << 24;
     a.bias = g.bias; a.add = g.add; a.ld_add = g.ld_add; a.pre = g.pre; a.ld_pre = g.ld_pre; a.out = g.out; a.ld_out = g.ld_out;
     a.scale = g.scale; a.act = g.act; a.accumulate = g.accumulate;
-    CUtensorMap maps[4] = {};
+    CUtensorMap maps[2] = {};
     const CUtensorMapDataType dt = type == B200RL_TYPE_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if((rc = make_map(&maps[0], dt, 2, A.p, matrix_rows(A, g.m, g.k), matrix_cols(A, g.m, g.k), A.ld, A.k_rows ? 64 : 128, 64, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
-    if((rc = make_map(&maps[1], dt, 2, B.p, matrix_rows(B, g.n, g.k), matrix_cols(B, g.n, g.k), B.ld, B.k_rows ? 64 : p.bn / p.cg, 64, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+    if((rc = make_map(&maps[0], dt, A.p, matrix_rows(A, g.m, g.k), matrix_cols(A, g.m, g.k), A.ld, A.k_rows ? 64 : 128))) return rc;
+    if((rc = make_map(&maps[1], dt, B.p, matrix_rows(B, g.n, g.k), matrix_cols(B, g.n, g.k), B.ld, B.k_rows ? 64 : p.bn / p.cg))) return rc;
     FinishArgs f{partial, p.ld_partial, p.ld_partial * (long long)g.m, p.splits, nullptr, a, g.row_sums};
     if(epilogue == EPI_SUM || p.partial){
         TcArgs b = a;
-        b.accumulate = p.partial ? 0 : g.accumulate;
-        float* out = p.partial ? partial : static_cast<float*>(g.out);
-        if((rc = make_map(&maps[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, out, g.m, g.n, p.partial ? p.ld_partial : g.ld_out, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, true, p.splits,
-                          f.split_stride))) return rc;
+        if(p.partial){ b.out = partial; b.ld_out = p.ld_partial; b.split_stride = f.split_stride; b.accumulate = 0; }
+        b.fast = rows_aligned(b.out, b.ld_out, 4);
         if(epilogue == EPI_SUM && g.row_sums){
             b.sum_source = A.p; b.ld_sum = A.ld;
             b.sums = p.splits > 1 ? reinterpret_cast<float*>(ws + p.off_sums) : g.row_sums;
@@ -767,12 +745,6 @@ static int product_tc_typed(const Product& g, int type, int epilogue, void* work
         return launch_finish<T, EPI_FORWARD>(f, s);
     }
     a.fast = rows_aligned(g.out, g.ld_out, 2) && (!g.add || rows_aligned(g.add, g.ld_add, 2)) && (!g.pre || rows_aligned(g.pre, g.ld_pre, 2));
-    if(a.fast){
-        const int width = p.bn / 2 < 64 ? p.bn / 2 : 64;                 // of a slab
-        const CUtensorMapSwizzle swizzle = width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-        if((rc = make_map(&maps[2], dt, 2, g.out, g.m, g.n, g.ld_out, 32, width, swizzle))) return rc;
-        if(epilogue == EPI_FORWARD && g.pre && (rc = make_map(&maps[3], dt, 2, g.pre, g.m, g.n, g.ld_pre, 32, width, swizzle))) return rc;
-    }
     if(epilogue == EPI_INPUT) return launch_tile<false, true, T, EPI_INPUT>(p, maps, a, s);
     return launch_tile<false, false, T, EPI_FORWARD>(p, maps, a, s);
 }

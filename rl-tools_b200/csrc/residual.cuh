@@ -47,27 +47,83 @@ template <typename T, int N> __device__ __forceinline__ void store_elements(T* p
     }
 }
 
+// Pairs of fp32 values: one instruction for both.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c){
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)), "l"(reinterpret_cast<const unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b){
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b){
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v){ return make_float2(v, v); }
+__device__ __forceinline__ float across(float2 v){ return v.x + v.y; }
+
 // Activations and their slopes: the framework's definitions and two more, with few instructions, since they run on every element that a product leaves (a tile of 128 x 256 over
 // 1024 k takes the tensor core 8,200 cycles; 256 threads that spend 45 instructions an element on erff take 11,500). Errors stay below 1e-6, a thousandth of the rounding to 16 bits.
 //   Phi(x): erfc by Abramowitz and Stegun, "Handbook of Mathematical Functions", 7.1.26: erfc(z) = t (a1 + t (a2 + ...)) exp(-z^2) within 1.5e-7, t = 1 / (1 + p z), z >= 0
-struct NormalTail { float phi, density; };                               // Phi(x) and exp(-x^2 / 2)
-__device__ __forceinline__ NormalTail normal_tail(float x){
-    const float z = fabsf(x) * 0.70710678118654752f, t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f)), density = __expf(-0.5f * x * x);
-    const float tail = 0.5f * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * density;
-    return {x < 0.0f ? tail : 1.0f - tail, density};
+// Phi(x) = 1/2 + sign(x) (1/2 - erfc(|x| / sqrt 2) / 2). Two at a time; the two reciprocals are one, of the product (|x| is cut at 20, where the density has long been 0).
+struct NormalPair { float2 phi, density; };                              // Phi(x) and exp(-x^2 / 2)
+__device__ __forceinline__ NormalPair normal_pair(float2 x){
+    const float2 d = fma2(make_float2(fminf(fabsf(x.x), 20.0f), fminf(fabsf(x.y), 20.0f)), both(0.3275911f * 0.70710678118654752f), both(1.0f));
+    const float r = __fdividef(1.0f, d.x * d.y);
+    const float2 t = mul2(make_float2(d.y, d.x), both(r));
+    const float2 e = mul2(mul2(x, x), both(-0.5f));
+    NormalPair n;
+    n.density = make_float2(__expf(e.x), __expf(e.y));
+    float2 p = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+    p = fma2(t, p, both(0.5f * 1.421413741f));
+    p = fma2(t, p, both(0.5f * -0.284496736f));
+    p = mul2(mul2(t, fma2(t, p, both(0.5f * 0.254829592f))), n.density);
+    const float2 off = fma2(p, both(-1.0f), both(0.5f));                  // >= 0 but for its last bits
+    n.phi = add2(make_float2(copysignf(off.x, x.x), copysignf(off.y, x.y)), both(0.5f));
+    return n;
 }
 __device__ __forceinline__ float fast_sigmoid(float x){ return __fdividef(1.0f, 1.0f + __expf(-x)); }      // exp(-x) = inf: 1 / inf = 0
 template <int ACT> __device__ __forceinline__ float residual_activation(float x){
-    if constexpr(ACT == B200RL_ACT_GELU) return x * normal_tail(x).phi;
+    if constexpr(ACT == B200RL_ACT_GELU) return x * normal_pair(both(x)).phi.x;
     else if constexpr(ACT == B200RL_ACT_SILU) return x * fast_sigmoid(x);
     else if constexpr(ACT == B200RL_ACT_SIGMOID) return fast_sigmoid(x);
     else return activation<ACT>(x);
 }
 template <int ACT> __device__ __forceinline__ float residual_d_activation(float x){
-    if constexpr(ACT == B200RL_ACT_GELU){ const NormalTail n = normal_tail(x); return fmaf(x * 0.39894228040143268f, n.density, n.phi); }
+    if constexpr(ACT == B200RL_ACT_GELU){ const NormalPair n = normal_pair(both(x)); return fmaf(x * 0.39894228040143268f, n.density.x, n.phi.x); }
     else if constexpr(ACT == B200RL_ACT_SILU){ const float s = fast_sigmoid(x); return s * fmaf(x, 1.0f - s, 1.0f); }
     else if constexpr(ACT == B200RL_ACT_SIGMOID){ const float s = fast_sigmoid(x); return s * (1.0f - s); }
     else return d_activation<ACT>(x);
+}
+// eight values in place; eight values times the slopes at eight places
+template <int ACT> __device__ __forceinline__ void activate8(float (&v)[8]){
+    if constexpr(ACT == B200RL_ACT_GELU)
+#pragma unroll
+        for(int c = 0; c < 8; c += 2){
+            const float2 x = make_float2(v[c], v[c + 1]), y = mul2(x, normal_pair(x).phi);
+            v[c] = y.x; v[c + 1] = y.y;
+        }
+    else
+#pragma unroll
+        for(int c = 0; c < 8; c++) v[c] = residual_activation<ACT>(v[c]);
+}
+template <int ACT> __device__ __forceinline__ void times_slope8(float (&v)[8], const float (&at)[8]){
+    if constexpr(ACT == B200RL_ACT_GELU)
+#pragma unroll
+        for(int c = 0; c < 8; c += 2){
+            const float2 x = make_float2(at[c], at[c + 1]);
+            const NormalPair n = normal_pair(x);
+            const float2 y = mul2(make_float2(v[c], v[c + 1]), fma2(mul2(x, both(0.39894228040143268f)), n.density, n.phi));
+            v[c] = y.x; v[c + 1] = y.y;
+        }
+    else
+#pragma unroll
+        for(int c = 0; c < 8; c++) v[c] *= residual_d_activation<ACT>(at[c]);
 }
 #define B200RL_DISPATCH_RESIDUAL_ACT(act, ...) \
     switch(act){ \
