@@ -60,7 +60,9 @@ using namespace b200rl;
 extern "C" {
 
 size_t b200rl_dense_residual_forward_workspace_bytes(const void* W, int ldw, const void* x, int ldx, int batch, int input_dim, int output_dim){
-    return batch < 1 || input_dim < 1 || output_dim < 1 ? 0 : product_tc_workspace_bytes(forward_product(W, ldw, x, ldx, batch, input_dim, output_dim), EPI_FORWARD);
+    if(batch < 1 || input_dim < 1 || output_dim < 1) return 0;
+    const Product g = forward_product(W, ldw, x, ldx, batch, input_dim, output_dim);
+    return product_rows_takes(g) ? 0 : product_tc_workspace_bytes(g, EPI_FORWARD);
 }
 size_t b200rl_dense_residual_backward_input_workspace_bytes(const void* W, int ldw, const void* d_pre, int ldd, int batch, int input_dim, int output_dim){
     return batch < 1 || input_dim < 1 || output_dim < 1 ? 0 : product_tc_workspace_bytes(input_product(W, ldw, d_pre, ldd, batch, input_dim, output_dim), EPI_INPUT);
@@ -79,13 +81,14 @@ int b200rl_dense_residual_forward(int type, const void* W, int ldw, const float*
        (residual && !valid_matrix(residual, ldr, batch, output_dim, 2)) || (pre && !valid_matrix(pre, ldpre, batch, output_dim, 2)) ||
        reinterpret_cast<uintptr_t>(bias) % 4) return B200RL_ERR_INVALID_ARGUMENT;
     Product g = forward_product(W, ldw, x, ldx, batch, input_dim, output_dim);
-    if(!valid_workspace(workspace, workspace_bytes, product_tc_workspace_bytes(g, EPI_FORWARD))) return B200RL_ERR_INVALID_ARGUMENT;
+    const bool few = product_rows_takes(g);
+    if(!few && !valid_workspace(workspace, workspace_bytes, product_tc_workspace_bytes(g, EPI_FORWARD))) return B200RL_ERR_INVALID_ARGUMENT;
     g.bias = bias; g.scale = scale;
     g.add = residual; g.ld_add = row_pitch(ldr, batch, output_dim);
     g.pre = pre; g.ld_pre = row_pitch(ldpre, batch, output_dim);
     g.out = y; g.ld_out = row_pitch(ldy, batch, output_dim);
     g.act = activation;
-    return product_tc(g, type, EPI_FORWARD, workspace, (cudaStream_t)stream);
+    return few ? product_rows(g, type, (cudaStream_t)stream) : product_tc(g, type, EPI_FORWARD, workspace, (cudaStream_t)stream);
 }
 
 int b200rl_dense_residual_backward_activation(int type, const void* pre, int ldpre, const void* d_y, int ldd, float scale, void* d_pre, int lddp, int rows,

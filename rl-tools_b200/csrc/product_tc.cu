@@ -12,6 +12,7 @@
 #include "tcgen05.cuh"
 #include <cuda.h>
 #include <atomic>
+#include <limits.h>
 
 namespace b200rl {
 
@@ -35,6 +36,7 @@ __device__ int g_product_tc_error = 0;                   // set when a bounded w
 struct TcArgs {
     int m, n, k;
     int m_tiles, n_tiles, splits, split_blocks;          // split_blocks: k blocks of 64 in a split
+    int cluster_splits;                                  // > 1: so many CTAs of a cluster share a tile, each with split_blocks of its k, and add up through one another's shared memory
     uint32_t idesc;
     const float* bias;
     const void* add; long long ld_add;
@@ -51,6 +53,12 @@ struct TcArgs {
 __device__ __forceinline__ uint32_t cluster_rank(){ uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t leader_address(const void* p){ uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(tc::smem_u32(p))); return r; }
 __device__ __forceinline__ void cluster_sync(){ asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float4 peer_load(uint32_t address){      // of a CTA of the cluster
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t peer_address(const void* p, uint32_t rank){ uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(tc::smem_u32(p)), "r"(rank)); return r; }
 __device__ __forceinline__ void arrive_expect(uint64_t* bar, uint32_t bytes){ asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(tc::smem_u32(bar)), "r"(bytes) : "memory"); }
 template <int CG> __device__ __forceinline__ void arrive_at_leader(uint64_t* bar){
     if constexpr(CG == 1) tc::mbar_arrive(bar);
@@ -205,6 +213,14 @@ __device__ __forceinline__ void finish_slab(const TcArgs& a, const uint8_t* slab
         if(there) store_chunk(out, pack_chunk<T>(v), elements);
     }
 }
+template <typename T, int EPI> __device__ __forceinline__ void finish_whole_or_part(const TcArgs& a, const uint8_t* slab, const SlabOperands& o, int row0, int col, int lane){
+    float bias[8];
+    if constexpr(EPI == EPI_FORWARD) if(a.bias)
+#pragma unroll
+        for(int c = 0; c < 8; c++) bias[c] = a.bias[min(col + 8 * (lane & 3) + c, a.n - 1)];
+    if(row0 + 32 <= a.m && col + 32 <= a.n){ B200RL_DISPATCH_RESIDUAL_ACT(a.act, (finish_slab<T, EPI, ACT, true>(a, slab, o, bias, row0, col, lane))) }
+    else { B200RL_DISPATCH_RESIDUAL_ACT(a.act, (finish_slab<T, EPI, ACT, false>(a, slab, o, bias, row0, col, lane))) }
+}
 // The same where rows start at odd addresses: a lane has a column
 template <typename T, int EPI>
 __device__ __forceinline__ void finish_slab_by_rows(const TcArgs& a, const uint8_t* slab, int row0, int col0, int lane){
@@ -277,7 +293,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
     float* sum_buffer = reinterpret_cast<float*>(slot + 4);                  // [2][SUM_COLUMNS]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0;                 // in a pair
+    const int sharers = CG == 1 && EPI != EPI_SUM ? a.cluster_splits : 1, share = sharers > 1 ? (int)cluster_rank() : 0;
     if(tid == 0){
         prefetch_map(&map_a); prefetch_map(&map_b);
         for(int s = 0; s < STAGES; s++){ tc::mbar_init(full + s, 1); tc::mbar_init(empty + s, 1); }
@@ -292,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     tc::fence_after_thread_sync();
     const uint32_t tmem = *slot;
     after_predecessor();
-    const int tiles = a.m_tiles * a.n_tiles * a.splits, first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
+    const int tiles = a.m_tiles * a.n_tiles * a.splits, first_tile = blockIdx.x / (CG * sharers), tile_step = gridDim.x / (CG * sharers);
     const int k_blocks = (a.k + KB - 1) / KB;
 
     if(warp < 4){
@@ -303,8 +320,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             for(int t = first_tile; t < tiles && ok; t += tile_step){
                 const TileIndex i = tile_index(a, t);
                 const int m0 = i.m * 128 * CG + (int)rank * 128, n0 = i.n * BN + (int)rank * (BN / CG);
-                const int kb_end = min(k_blocks, (i.z + 1) * a.split_blocks);
-                for(int kb = i.z * a.split_blocks; kb < kb_end; kb++, it++){
+                const int part = i.z + share, kb_end = min(k_blocks, (part + 1) * a.split_blocks);
+                for(int kb = part * a.split_blocks; kb < kb_end; kb++, it++){
                     const uint32_t s = it % STAGES, phase = (it / STAGES) & 1;
                     if(!tc::mbar_wait_bounded(empty + s, phase ^ 1, WAIT_LIMIT) || *abort_flag){ ok = false; break; }
                     uint8_t* stage = base + s * STAGE;
@@ -332,9 +349,9 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             uint32_t it = 0, acc = 0;
             bool ok = true;
             for(int t = first_tile; t < tiles && ok; t += tile_step){
-                const int z = t / (a.m_tiles * a.n_tiles);
-                const int kb_end = min(k_blocks, (z + 1) * a.split_blocks);
-                for(int kb0 = z * a.split_blocks; kb0 < kb_end && ok; acc++){
+                const int part = t / (a.m_tiles * a.n_tiles) + share;
+                const int kb_end = min(k_blocks, (part + 1) * a.split_blocks);
+                for(int kb0 = part * a.split_blocks; kb0 < kb_end && ok; acc++){
                     const int piece_end = EPI == EPI_SUM ? min(kb_end, kb0 + PIECE / KB) : kb_end;
                     const uint32_t b = acc & 1, d = tmem + b * BN;
                     if(!tc::mbar_wait_bounded(acc_empty + b, ((acc >> 1) & 1) ^ 1, WAIT_LIMIT)){ ok = false; break; }
@@ -360,6 +377,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         }
         else if(EPI == EPI_SUM && warp >= 2 && a.sums) sum_rows<T>(a, sum_buffer, tid - 64, warp - 2, lane);
         __syncwarp();
+        if constexpr(CG == 1 && EPI != EPI_SUM) if(sharers > 1){ cluster_sync(); cluster_sync(); }       // as the epilogue warps do
     }
     else{
         tc::setmaxnreg_inc<104>();
@@ -415,10 +433,19 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 const uint32_t b = acc & 1, phase = (acc >> 1) & 1;
                 acc++;
                 SlabOperands o;
-                if(a.fast) fetch_slab<T, EPI>(o, a, row0, col0, lane);
+                if(a.fast && sharers == 1) fetch_slab<T, EPI>(o, a, row0, col0, lane);
                 if(!tc::mbar_wait_bounded(acc_full + b, phase, WAIT_LIMIT)){ ok = false; break; }
                 tc::fence_after_thread_sync();
                 uint32_t r[32];
+                if(sharers > 1){                                         // one tile a cluster: its sums go where the operands were
+#pragma unroll
+                    for(int j = 0; j < SLABS; j++){
+                        tc::tmem_ld_32x32(tmem + lanes + b * BN + group * CW + j * 32, r);
+                        tc::tmem_wait_ld();
+                        slab_in(base + (w * SLABS + j) * 4096, r, lane);
+                    }
+                    break;
+                }
                 tc::tmem_ld_32x32(tmem + lanes + b * BN + group * CW, r);
 #pragma unroll 1
                 for(int j = 0; j < SLABS; j++){
@@ -432,18 +459,50 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     if(j + 1 == SLABS && lane == 0) arrive_at_leader<CG>(acc_empty + b);
                     if(row0 >= a.m || col >= a.n) continue;
                     if(!a.fast){ finish_slab_by_rows<T, EPI>(a, slab, row0, col, lane); continue; }
-                    float bias[8];
-                    if constexpr(EPI == EPI_FORWARD) if(a.bias)
-#pragma unroll
-                        for(int c = 0; c < 8; c++) bias[c] = a.bias[min(col + 8 * (lane & 3) + c, a.n - 1)];
-                    if(row0 + 32 <= a.m && col + 32 <= a.n){ B200RL_DISPATCH_RESIDUAL_ACT(a.act, (finish_slab<T, EPI, ACT, true>(a, slab, o, bias, row0, col, lane))) }
-                    else { B200RL_DISPATCH_RESIDUAL_ACT(a.act, (finish_slab<T, EPI, ACT, false>(a, slab, o, bias, row0, col, lane))) }
+                    finish_whole_or_part<T, EPI>(a, slab, o, row0, col, lane);
                     if(j + 1 < SLABS) fetch_slab<T, EPI>(o, a, row0, col + 32, lane);
                 }
             }
         }
         if(!ok){ *abort_flag = 1; g_product_tc_error = 1; }
         __syncwarp();
+        if constexpr(CG == 1 && EPI != EPI_SUM) if(sharers > 1){
+            // every CTA's sums are in place; each takes every so many-th slab, adds up the shares in their order and finishes it
+            const TileIndex i = tile_index(a, first_tile);
+            const int row0 = i.m * 128 + q * 32;
+            const bool works = group < GROUPS && row0 < a.m;
+            cluster_sync();
+            if(works)
+#pragma unroll 1
+                for(int j = 0; j < SLABS; j++){
+                    const int col = i.n * BN + group * CW + j * 32;
+                    if((w * SLABS + j) % sharers != share || col >= a.n) continue;
+                    SlabOperands o;
+                    if(a.fast) fetch_slab<T, EPI>(o, a, row0, col, lane);
+                    uint8_t* slab = staging + w * STAGING;
+                    __syncwarp();
+#pragma unroll 1
+                    for(int half = 0; half < 2; half++){
+                        float4 sum[4];
+                        for(int s = 0; s < sharers; s++){
+                            const uint32_t from = peer_address(base + (w * SLABS + j) * 4096 + half * 2048, s);
+#pragma unroll
+                            for(int c = 0; c < 4; c++){
+                                const float4 v = peer_load(from + (c * 32 + lane) * 16);
+                                if(s == 0) sum[c] = v;
+                                else { sum[c].x += v.x; sum[c].y += v.y; sum[c].z += v.z; sum[c].w += v.w; }
+                            }
+                        }
+#pragma unroll
+                        for(int c = 0; c < 4; c++) *reinterpret_cast<float4*>(slab + half * 2048 + (c * 32 + lane) * 16) = sum[c];
+                    }
+                    __syncwarp();
+                    if(a.fast) finish_whole_or_part<T, EPI>(a, slab, o, row0, col, lane);
+                    else finish_slab_by_rows<T, EPI>(a, slab, row0, col, lane);
+                }
+            __syncwarp();
+            cluster_sync();                                                  // no CTA leaves while its sums are read
+        }
     }
     tc::fence_before_thread_sync();
     __syncthreads();
@@ -519,8 +578,7 @@ struct FinishArgs {
     TcArgs a;
     float* sums;
 };
-// out = epilogue(sum over the splits, in their order), a thread an element
-template <typename T, int EPI>
+// out (+)= sum over the splits, in their order, a thread an element
 __global__ void __launch_bounds__(256) finish_kernel(FinishArgs f){
     after_predecessor();
     const TcArgs& a = f.a;
@@ -529,30 +587,12 @@ __global__ void __launch_bounds__(256) finish_kernel(FinishArgs f){
         const long long row = i / a.n; const int col = (int)(i - row * a.n);
         const float* p = f.partial + row * f.ld_partial + col;
         float x = 0.0f;
+#pragma unroll 4
         for(int z = 0; z < f.splits; z++) x += p[z * f.split_stride];
-        if constexpr(EPI == EPI_SUM){
-            float* out = static_cast<float*>(a.out) + row * a.ld_out + col;
-            *out = a.accumulate ? *out + x : x;
-        }
-        else{
-            const float add = a.add ? to_float(static_cast<const T*>(a.add)[row * a.ld_add + col]) : 0.0f;
-            if constexpr(EPI == EPI_FORWARD){
-                if(a.bias) x += a.bias[col];
-                if(a.pre) static_cast<T*>(a.pre)[row * a.ld_pre + col] = from_float<T>(x);
-                B200RL_DISPATCH_RESIDUAL_ACT(a.act, x = residual_activation<ACT>(x))
-                x = fmaf(a.scale, x, add);
-            }
-            else{
-                x += add;
-                if(a.act != B200RL_ACT_IDENTITY){
-                    const float q = to_float(static_cast<const T*>(a.pre)[row * a.ld_pre + col]);
-                    B200RL_DISPATCH_RESIDUAL_ACT(a.act, x *= residual_d_activation<ACT>(q))
-                }
-            }
-            static_cast<T*>(a.out)[row * a.ld_out + col] = from_float<T>(x);
-        }
+        float* out = static_cast<float*>(a.out) + row * a.ld_out + col;
+        *out = a.accumulate ? *out + x : x;
     }
-    if constexpr(EPI == EPI_SUM) if(f.row_sums)
+    if(f.row_sums)
         for(int r = blockIdx.x * 256 + threadIdx.x; r < a.m; r += gridDim.x * 256){
             float x = 0.0f;
             for(int z = 0; z < f.splits; z++) x += f.row_sums[(long long)z * a.m + r];
@@ -605,7 +645,7 @@ static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, l
 }
 
 struct TcPlan {
-    int cg, bn, m_tiles, n_tiles, splits, split_blocks;
+    int cg, bn, m_tiles, n_tiles, splits, split_blocks, cluster_splits;
     bool copy_a, copy_b, partial;
     long long ld_copy_a, ld_copy_b, ld_partial;
     size_t off_b, off_partial, off_sums, bytes;
@@ -615,21 +655,38 @@ static long long matrix_cols(const Operand& o, int r, int k){ return o.k_rows ? 
 static TcPlan plan_product(const Product& g, int epilogue){
     TcPlan p{};
     const int k_blocks = (g.k + KB - 1) / KB;
-    auto tiles_of = [&](int cg, int bn){ return (long long)((g.m + 128 * cg - 1) / (128 * cg)) * ((g.n + bn - 1) / bn); };
-    if(tiles_of(2, 256) >= NUM_SMS / 2 - 10) { p.cg = 2; p.bn = 256; }
-    else if(tiles_of(1, 128) >= NUM_SMS - 20) { p.cg = 1; p.bn = 128; }
-    else { p.cg = 1; p.bn = 64; }
-    p.m_tiles = (g.m + 128 * p.cg - 1) / (128 * p.cg);
-    p.n_tiles = (g.n + p.bn - 1) / p.bn;
-    const long long tiles = (long long)p.m_tiles * p.n_tiles;
-    const int most = (k_blocks + PIECE / KB - 1) / (PIECE / KB);
-    p.splits = 1;
-    if(tiles * p.cg * 2 <= NUM_SMS){
-        p.splits = (int)(NUM_SMS / (tiles * p.cg));
-        if(p.splits > most) p.splits = most;
+    // Shape of the tiles and shares of k, by the cycles that a CTA needs: for a block of 64 k the bytes of its stage at the 48 a cycle that L2 gives a multiprocessor when all ask
+    // (measured; the MMAs take 128 to 512), for a tile 1,500 until its sums are out, for a shared tile 2,500 more. Sharing a tile needs a CTA for each share at the same time.
+    double best = 0.0;
+    for(int option = 0; option < 3; option++){
+        const int cg = option == 2 ? 2 : 1, bn = option == 0 ? 64 : option == 1 ? 128 : 256, groups = NUM_SMS / cg;
+        const long long m_tiles = (g.m - 1) / (128 * cg) + 1, n_tiles = (g.n - 1) / bn + 1, tiles = m_tiles * n_tiles;
+        if(tiles > INT_MAX / 64) continue;
+        const double block = stage_bytes(cg, bn) / 48.0;
+        for(int shares = 1; shares <= (cg == 1 ? 8 : 1); shares *= 2){
+            const bool by_cluster = epilogue != EPI_SUM;
+            const int most = by_cluster ? (shares == 8 ? 15 : shares == 4 ? 33 : 74) : NUM_SMS / shares;     // clusters that are resident together
+            if(shares > 1 && (tiles > most || k_blocks < 2 * shares)) break;
+            const int blocks = (k_blocks - 1) / shares + 1;
+            const double cycles = (double)((tiles * shares - 1) / groups + 1) * (blocks * block + 1500.0) + (shares > 1 ? 2500.0 : 0.0);
+            if(best == 0.0 || cycles < best){
+                best = cycles;
+                p.cg = cg; p.bn = bn; p.m_tiles = (int)m_tiles; p.n_tiles = (int)n_tiles; p.split_blocks = blocks;
+                p.splits = by_cluster ? 1 : (k_blocks - 1) / blocks + 1;
+                p.cluster_splits = by_cluster ? (k_blocks - 1) / blocks + 1 : 1;
+            }
+        }
     }
-    p.split_blocks = (k_blocks + p.splits - 1) / p.splits;
-    p.splits = (k_blocks + p.split_blocks - 1) / p.split_blocks;
+    if(epilogue == EPI_SUM && p.cg == 1){
+        // long sums of few tiles: as many splits as fill the device, a piece each at the least
+        const long long tiles = (long long)p.m_tiles * p.n_tiles;
+        const long long most = (k_blocks - 1) / (PIECE / KB) + 1, fill = NUM_SMS / tiles;
+        const long long splits = fill < most ? fill : most;
+        if(splits > p.splits){
+            p.split_blocks = (int)((k_blocks - 1) / splits + 1);
+            p.splits = (k_blocks - 1) / p.split_blocks + 1;
+        }
+    }
     // operands that TMA cannot address are copied
     p.copy_a = !rows_aligned(g.a.p, g.a.ld, 2) && !(matrix_rows(g.a, g.m, g.k) <= 1 && reinterpret_cast<uintptr_t>(g.a.p) % 16 == 0);
     p.copy_b = !rows_aligned(g.b.p, g.b.ld, 2) && !(matrix_rows(g.b, g.n, g.k) <= 1 && reinterpret_cast<uintptr_t>(g.b.p) % 16 == 0);
@@ -664,7 +721,8 @@ static int launch_tc(const CUtensorMap (&maps)[2], const TcArgs& a, cudaStream_t
     if(rc || (rc = sm_count(&sms))) return rc;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    const int cluster = CG * a.cluster_splits;
+    attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.blockDim = THREADS; cfg.dynamicSmemBytes = smem_bytes(CG, BN); cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = 1;
     int most = groups[dev].load(std::memory_order_acquire);
@@ -678,8 +736,9 @@ static int launch_tc(const CUtensorMap (&maps)[2], const TcArgs& a, cudaStream_t
         }
         groups[dev].store(most, std::memory_order_release);
     }
+    // a tile that is shared has a cluster of its own; else as many CTAs (or pairs) as run at the same time take the tiles in turn
     const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
-    cfg.gridDim = (unsigned)(CG * (tiles < most ? tiles : most));
+    cfg.gridDim = (unsigned)(a.cluster_splits > 1 ? tiles * cluster : CG * (tiles < most ? tiles : most));
     cfg.numAttrs = 2;
     B200RL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], a));
     return B200RL_OK;
@@ -690,10 +749,9 @@ static int launch_tile(const TcPlan& p, const CUtensorMap (&maps)[2], const TcAr
     if(p.bn == 128) return launch_tc<1, 128, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
     return launch_tc<1, 64, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
 }
-template <typename T, int EPI>
 static int launch_finish(const FinishArgs& f, cudaStream_t s){
     const long long blocks = ((long long)f.a.m * f.a.n + 255) / 256;
-    B200RL_CUDA_TRY(launch_after(finish_kernel<T, EPI>, dim3((unsigned)(blocks < NUM_SMS * 8 ? blocks : NUM_SMS * 8)), dim3(256), 0, s, f));
+    B200RL_CUDA_TRY(launch_after(finish_kernel, dim3((unsigned)(blocks < NUM_SMS * 8 ? blocks : NUM_SMS * 8)), dim3(256), 0, s, f));
     return B200RL_OK;
 }
 
@@ -714,7 +772,7 @@ static int product_tc_typed(const Product& g, int type, int epilogue, void* work
     float* partial = reinterpret_cast<float*>(ws + p.off_partial);
     TcArgs a{};
     a.m = g.m; a.n = g.n; a.k = g.k;
-    a.m_tiles = p.m_tiles; a.n_tiles = p.n_tiles; a.splits = p.splits; a.split_blocks = p.split_blocks;
+    a.m_tiles = p.m_tiles; a.n_tiles = p.n_tiles; a.splits = p.splits; a.split_blocks = p.split_blocks; a.cluster_splits = p.cluster_splits;
     const uint32_t format = type == B200RL_TYPE_BFLOAT16 ? 1u : 0u;
     // fp32 sums, both operands of one type, their k_rows forms, N / 8, M / 16
     a.idesc = 1u << 4 | format << 7 | format << 10 | (A.k_rows ? 1u << 15 : 0u) | (B.k_rows ? 1u << 16 : 0u) | (uint32_t)(p.bn / 8) << 17 | (uint32_t)(128 * p.cg / 16) << 24;
@@ -725,24 +783,19 @@ static int product_tc_typed(const Product& g, int type, int epilogue, void* work
     if((rc = make_map(&maps[0], dt, A.p, matrix_rows(A, g.m, g.k), matrix_cols(A, g.m, g.k), A.ld, A.k_rows ? 64 : 128))) return rc;
     if((rc = make_map(&maps[1], dt, B.p, matrix_rows(B, g.n, g.k), matrix_cols(B, g.n, g.k), B.ld, B.k_rows ? 64 : p.bn / p.cg))) return rc;
     FinishArgs f{partial, p.ld_partial, p.ld_partial * (long long)g.m, p.splits, nullptr, a, g.row_sums};
-    if(epilogue == EPI_SUM || p.partial){
+    if(epilogue == EPI_SUM){
         TcArgs b = a;
         if(p.partial){ b.out = partial; b.ld_out = p.ld_partial; b.split_stride = f.split_stride; b.accumulate = 0; }
         b.fast = rows_aligned(b.out, b.ld_out, 4);
-        if(epilogue == EPI_SUM && g.row_sums){
+        if(g.row_sums){
             b.sum_source = A.p; b.ld_sum = A.ld;
             b.sums = p.splits > 1 ? reinterpret_cast<float*>(ws + p.off_sums) : g.row_sums;
             b.sums_accumulate = p.splits > 1 ? 0 : g.accumulate;
             f.row_sums = p.splits > 1 ? b.sums : nullptr;
             f.a.sums_accumulate = g.accumulate;
         }
-        if(A.k_rows && B.k_rows) rc = launch_tile<true, true, T, EPI_SUM>(p, maps, b, s);
-        else if(B.k_rows) rc = launch_tile<false, true, T, EPI_SUM>(p, maps, b, s);
-        else rc = launch_tile<false, false, T, EPI_SUM>(p, maps, b, s);
-        if(rc || !p.partial) return rc;
-        if(epilogue == EPI_SUM) return launch_finish<T, EPI_SUM>(f, s);
-        if(epilogue == EPI_INPUT) return launch_finish<T, EPI_INPUT>(f, s);
-        return launch_finish<T, EPI_FORWARD>(f, s);
+        if((rc = launch_tile<true, true, T, EPI_SUM>(p, maps, b, s)) || !p.partial) return rc;
+        return launch_finish(f, s);
     }
     a.fast = rows_aligned(g.out, g.ld_out, 2) && (!g.add || rows_aligned(g.add, g.ld_add, 2)) && (!g.pre || rows_aligned(g.pre, g.ld_pre, 2));
     if(epilogue == EPI_INPUT) return launch_tile<false, true, T, EPI_INPUT>(p, maps, a, s);

@@ -34,7 +34,7 @@ def seeded(n):
 # sizes: one token, a few, tiles and their neighbours, odd depths, depths of one element; the largest are small enough for a 64-bit product in milliseconds
 DENSE_SIZES = [(1, 1, 1), (1, 64, 256), (1, 1024, 777), (2, 17, 5), (5, 250, 131), (8, 512, 512), (16, 4096, 33), (31, 77, 129), (33, 264, 136), (64, 256, 1024), (65, 128, 64),
                (127, 63, 255), (128, 64, 256), (129, 65, 257), (200, 1000, 320), (256, 256, 256), (300, 40, 1111), (513, 640, 384), (1003, 777, 1001), (2048, 512, 768), (4100, 72, 40),
-               (16400, 72, 300), (5003, 200, 1000), (1100, 2050, 2100)]
+               (16400, 72, 300), (5003, 200, 1000), (1100, 2050, 2100), (128, 4096, 96), (33, 4000, 520), (100, 1030, 1000), (260, 2000, 250)]
 
 
 def dense_inputs(B, I, O, dtype, pad, offset, seed):
