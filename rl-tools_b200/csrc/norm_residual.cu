@@ -414,29 +414,47 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, backward_ctas<T>(TPR, E
 #pragma unroll
         for(int i = 0; i < P; i++){ d[i] = mul2(d[i], both(a.scale)); u[i] = mul2(u[i], both(rstd_u)); }
         if constexpr(GATE) if(gated){
-            if(a.d_gate){
-                float b[E];
-                if(BIAS && post) row.parameters(a.post_bias, 0.0f, b);
+            const bool group_ends = r + 1 == group_end, flush = group_ends || r + 1 == last;
+            if constexpr(BIAS){
+                if(a.d_gate){
+                    float b[E];
+                    if(post) row.parameters(a.post_bias, 0.0f, b);
 #pragma unroll
-                for(int i = 0; i < E / 4; i++){
-                    float2 v0 = u[2 * i], v1 = u[2 * i + 1];
-                    if(post){
-                        const float4 w = kept.at(K::POST_WEIGHT, i);
-                        v0 = fma2(v0, make_float2(w.x, w.y), BIAS ? make_float2(b[4 * i], b[4 * i + 1]) : both(0.0f));
-                        v1 = fma2(v1, make_float2(w.z, w.w), BIAS ? make_float2(b[4 * i + 2], b[4 * i + 3]) : both(0.0f));
+                    for(int i = 0; i < E / 4; i++){
+                        float2 v0 = u[2 * i], v1 = u[2 * i + 1];
+                        if(post){
+                            const float4 w = kept.at(K::POST_WEIGHT, i);
+                            v0 = fma2(v0, make_float2(w.x, w.y), make_float2(b[4 * i], b[4 * i + 1]));
+                            v1 = fma2(v1, make_float2(w.z, w.w), make_float2(b[4 * i + 2], b[4 * i + 3]));
+                        }
+                        add_to(K::SUM_GATE, i, d[2 * i], v0, d[2 * i + 1], v1);
                     }
-                    add_to(K::SUM_GATE, i, d[2 * i], v0, d[2 * i + 1], v1);
                 }
-                const bool ends = r + 1 == group_end;
-                if(ends || r + 1 == last){
-                    // the gate row's sum is complete here, or a piece of it: the group's rows go on with the next worker, or began with one before
-                    float sum[E];
-                    hand_out(K::SUM_GATE, sum);
-                    if(ends && group_begin >= first) row.store(a.d_gate, group * a.lddg, sum);
-                    else row.store_sums(a.pieces + ((long long)worker * 2 + (group_begin >= first ? 1 : 0)) * a.dim, sum);
+            }
+            else
 #pragma unroll
-                    for(int i = 0; i < E / 4; i++) kept.at(K::SUM_GATE, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for(int i = 0; i < E / 4; i++) add_to(K::SUM_GATE, i, d[2 * i], u[2 * i], d[2 * i + 1], u[2 * i + 1]);
+            if(flush){
+                float sum[E];
+                hand_out(K::SUM_GATE, sum);
+                if constexpr(!BIAS) if(post)
+                    // without biases one sum of d u over the group gives both gradients: weight times it the gate's, gate times it the weight's
+#pragma unroll
+                    for(int i = 0; i < E / 4; i++){
+                        const float4 w = kept.at(K::POST_WEIGHT, i);
+                        float4 t = kept.at(K::SUM_POST_WEIGHT, i);
+                        t.x = fmaf(to_float(raw_gate.e[4 * i]), sum[4 * i], t.x); t.y = fmaf(to_float(raw_gate.e[4 * i + 1]), sum[4 * i + 1], t.y);
+                        t.z = fmaf(to_float(raw_gate.e[4 * i + 2]), sum[4 * i + 2], t.z); t.w = fmaf(to_float(raw_gate.e[4 * i + 3]), sum[4 * i + 3], t.w);
+                        kept.at(K::SUM_POST_WEIGHT, i) = t;
+                        sum[4 * i] *= w.x; sum[4 * i + 1] *= w.y; sum[4 * i + 2] *= w.z; sum[4 * i + 3] *= w.w;
+                    }
+                if(a.d_gate){
+                    // the gate row's sum is complete here, or a piece of it: the group's rows go on with the next worker, or began with one before
+                    if(group_ends && group_begin >= first) row.store(a.d_gate, group * a.lddg, sum);
+                    else row.store_sums(a.pieces + ((long long)worker * 2 + (group_begin >= first ? 1 : 0)) * a.dim, sum);
                 }
+#pragma unroll
+                for(int i = 0; i < E / 4; i++) kept.at(K::SUM_GATE, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
 #pragma unroll
             for(int i = 0; i < P; i++) d[i] = mul2(d[i], make_float2(to_float(raw_gate.e[2 * i]), to_float(raw_gate.e[2 * i + 1])));
@@ -452,7 +470,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, backward_ctas<T>(TPR, E
 #pragma unroll
             for(int i = 0; i < E / 4; i++){
                 const float4 w = kept.at(K::POST_WEIGHT, i);
-                add_to(K::SUM_POST_WEIGHT, i, d[2 * i], u[2 * i], d[2 * i + 1], u[2 * i + 1]);
+                if(BIAS || !GATE) add_to(K::SUM_POST_WEIGHT, i, d[2 * i], u[2 * i], d[2 * i + 1], u[2 * i + 1]);
                 if constexpr(BIAS) add_to(K::SUM_POST_BIAS, i, d[2 * i], both(1.0f), d[2 * i + 1], both(1.0f));
                 d[2 * i] = mul2(d[2 * i], make_float2(w.x, w.y));
                 d[2 * i + 1] = mul2(d[2 * i + 1], make_float2(w.z, w.w));

@@ -36,8 +36,9 @@ __device__ int g_product_tc_error = 0;                   // set when a bounded w
 struct TcArgs {
     int m, n, k;
     int m_tiles, n_tiles, splits, split_blocks;          // split_blocks: k blocks of 64 in a split
+    int whole_tiles;                                     // tiles from here on are taken in two halves of BN / 2 columns (CG == 2)
     int cluster_splits;                                  // > 1: so many CTAs of a cluster share a tile, each with split_blocks of its k, and add up through one another's shared memory
-    uint32_t idesc;
+    uint32_t idesc, idesc_half;
     const float* bias;
     const void* add; long long ld_add;
     void* pre; long long ld_pre;
@@ -101,10 +102,13 @@ __device__ __forceinline__ uint64_t make_desc_rows_sw128(uint32_t smem_addr){
     return (uint64_t)((smem_addr >> 4) & 0x3FFF) | (uint64_t)(8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-struct TileIndex { int m, n, z; };
-// tiles in groups of eight rows of tiles, along the rows first: what runs at the same time shares operands in L2
+struct TileIndex { int m, n, z, half; };                 // half: -1 a whole tile, 0 or 1 a half of it
+// Tiles in groups of eight rows of tiles, along the rows first: what runs at the same time shares operands in L2. Behind the whole tiles come those of the last round, in halves
+// where that lets twice as many pairs of CTAs work on them.
 __device__ __forceinline__ TileIndex tile_index(const TcArgs& a, int t){
     TileIndex i;
+    i.half = -1;
+    if(t >= a.whole_tiles){ i.half = (t - a.whole_tiles) & 1; t = a.whole_tiles + ((t - a.whole_tiles) >> 1); }
     const int per_split = a.m_tiles * a.n_tiles;
     i.z = t / per_split; t -= i.z * per_split;
     const int group = t / (8 * a.n_tiles), first = group * 8, rows = min(8, a.m_tiles - first);
@@ -228,25 +232,32 @@ __device__ __forceinline__ void finish_slab_by_rows(const TcArgs& a, const uint8
     if(col >= a.n) return;
     const float bias = EPI == EPI_FORWARD && a.bias ? a.bias[col] : 0.0f;
     const int rows = min(32, a.m - row0);
-#pragma unroll 4
-    for(int r = 0; r < rows; r++){
-        const long long row = row0 + r;
-        float x = slab_element(slab, r, lane);
-        const float add = a.add ? to_float(static_cast<const T*>(a.add)[row * a.ld_add + col]) : 0.0f;
+#pragma unroll 1
+    for(int r0 = 0; r0 < rows; r0 += 8){
+        float add[8], x[8];                                              // eight rows' operands under way together
+#pragma unroll
+        for(int r = 0; r < 8; r++) add[r] = a.add && r0 + r < rows ? to_float(static_cast<const T*>(a.add)[(long long)(row0 + r0 + r) * a.ld_add + col]) : 0.0f;
+#pragma unroll
+        for(int r = 0; r < 8; r++) x[r] = slab_element(slab, r0 + r, lane) + bias;
         if constexpr(EPI == EPI_FORWARD){
-            x += bias;
-            if(a.pre) static_cast<T*>(a.pre)[row * a.ld_pre + col] = from_float<T>(x);
-            B200RL_DISPATCH_RESIDUAL_ACT(a.act, x = residual_activation<ACT>(x))
-            x = fmaf(a.scale, x, add);
+            if(a.pre)
+#pragma unroll
+                for(int r = 0; r < 8; r++) if(r0 + r < rows) static_cast<T*>(a.pre)[(long long)(row0 + r0 + r) * a.ld_pre + col] = from_float<T>(x[r]);
+            B200RL_DISPATCH_RESIDUAL_ACT(a.act, activate8<ACT>(x))
+#pragma unroll
+            for(int r = 0; r < 8; r++) x[r] = fmaf(a.scale, x[r], add[r]);
         }
         else{
-            x += add;
+#pragma unroll
+            for(int r = 0; r < 8; r++) x[r] += add[r];
             if(a.act != B200RL_ACT_IDENTITY){
-                const float p = to_float(static_cast<const T*>(a.pre)[row * a.ld_pre + col]);
-                B200RL_DISPATCH_RESIDUAL_ACT(a.act, x *= residual_d_activation<ACT>(p))
+#pragma unroll
+                for(int r = 0; r < 8; r++) add[r] = r0 + r < rows ? to_float(static_cast<const T*>(a.pre)[(long long)(row0 + r0 + r) * a.ld_pre + col]) : 0.0f;
+                B200RL_DISPATCH_RESIDUAL_ACT(a.act, times_slope8<ACT>(x, add))
             }
         }
-        static_cast<T*>(a.out)[row * a.ld_out + col] = from_float<T>(x);
+#pragma unroll
+        for(int r = 0; r < 8; r++) if(r0 + r < rows) static_cast<T*>(a.out)[(long long)(row0 + r0 + r) * a.ld_out + col] = from_float<T>(x[r]);
     }
 }
 // A slab of an fp32 result
@@ -309,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     tc::fence_after_thread_sync();
     const uint32_t tmem = *slot;
     after_predecessor();
-    const int tiles = a.m_tiles * a.n_tiles * a.splits, first_tile = blockIdx.x / (CG * sharers), tile_step = gridDim.x / (CG * sharers);
+    const int all = a.m_tiles * a.n_tiles * a.splits, tiles = CG == 2 ? a.whole_tiles + 2 * (all - a.whole_tiles) : all, first_tile = blockIdx.x / (CG * sharers), tile_step = gridDim.x / (CG * sharers);
     const int k_blocks = (a.k + KB - 1) / KB;
 
     if(warp < 4){
@@ -319,23 +330,26 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             bool ok = true;
             for(int t = first_tile; t < tiles && ok; t += tile_step){
                 const TileIndex i = tile_index(a, t);
-                const int m0 = i.m * 128 * CG + (int)rank * 128, n0 = i.n * BN + (int)rank * (BN / CG);
+                const bool half = CG == 2 && i.half >= 0;
+                const int m0 = i.m * 128 * CG + (int)rank * 128, n0 = i.n * BN + (half ? i.half * (BN / 2) + (int)rank * (BN / CG / 2) : (int)rank * (BN / CG));
+                const uint32_t bytes = half ? STAGE - (STAGE - A_BYTES) / 2 : STAGE;
                 const int part = i.z + share, kb_end = min(k_blocks, (part + 1) * a.split_blocks);
                 for(int kb = part * a.split_blocks; kb < kb_end; kb++, it++){
                     const uint32_t s = it % STAGES, phase = (it / STAGES) & 1;
                     if(!tc::mbar_wait_bounded(empty + s, phase ^ 1, WAIT_LIMIT) || *abort_flag){ ok = false; break; }
                     uint8_t* stage = base + s * STAGE;
-                    if(rank == 0) arrive_expect(full + s, CG * STAGE);
+                    if(rank == 0) arrive_expect(full + s, CG * bytes);
                     if constexpr(A_ROWS){
                         load_box<CG>(stage, &map_a, m0, kb * KB, full + s);
                         load_box<CG>(stage + 8192, &map_a, m0 + 64, kb * KB, full + s);
                     }
                     else load_box<CG>(stage, &map_a, kb * KB, m0, full + s);
-                    if constexpr(B_ROWS){
 #pragma unroll
-                        for(int j = 0; j < BN / CG / 64; j++) load_box<CG>(stage + A_BYTES + j * 8192, &map_b, n0 + 64 * j, kb * KB, full + s);
+                    for(int j = 0; j < BN / CG / 64; j++){                // boxes of 64 rows of B either way
+                        if(j >= BN / CG / 128 && half) break;
+                        if constexpr(B_ROWS) load_box<CG>(stage + A_BYTES + j * 8192, &map_b, n0 + 64 * j, kb * KB, full + s);
+                        else load_box<CG>(stage + A_BYTES + j * 8192, &map_b, kb * KB, n0 + 64 * j, full + s);
                     }
-                    else load_box<CG>(stage + A_BYTES, &map_b, kb * KB, n0, full + s);
                 }
             }
             // no CTA leaves while its copies or its peer's signals are under way: the last use of every stage has been released
@@ -349,7 +363,9 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             uint32_t it = 0, acc = 0;
             bool ok = true;
             for(int t = first_tile; t < tiles && ok; t += tile_step){
-                const int part = t / (a.m_tiles * a.n_tiles) + share;
+                const TileIndex i = tile_index(a, t);
+                const int part = i.z + share;
+                const uint32_t idesc = CG == 2 && i.half >= 0 ? a.idesc_half : a.idesc;
                 const int kb_end = min(k_blocks, (part + 1) * a.split_blocks);
                 for(int kb0 = part * a.split_blocks; kb0 < kb_end && ok; acc++){
                     const int piece_end = EPI == EPI_SUM ? min(kb_end, kb0 + PIECE / KB) : kb_end;
@@ -365,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                         const uint64_t db = B_ROWS ? make_desc_rows_sw128(stage + A_BYTES) : tc::make_desc_kmajor_sw128(stage + A_BYTES);
 #pragma unroll
                         for(int ks = 0; ks < KB / 16; ks++)
-                            mma<CG>(d, da + (uint64_t)(ks * (A_ROWS ? 128 : 2)), db + (uint64_t)(ks * (B_ROWS ? 128 : 2)), a.idesc, (kb > kb0 || ks) ? 1u : 0u);
+                            mma<CG>(d, da + (uint64_t)(ks * (A_ROWS ? 128 : 2)), db + (uint64_t)(ks * (B_ROWS ? 128 : 2)), idesc, (kb > kb0 || ks) ? 1u : 0u);
                         commit<CG>(empty + s);
                     }
                     if(!ok) break;
@@ -388,7 +404,9 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         bool ok = true;
         for(int t = first_tile; t < tiles && ok && group < GROUPS; t += tile_step){
             const TileIndex i = tile_index(a, t);
-            const int row0 = i.m * 128 * CG + (int)rank * 128 + q * 32, col0 = i.n * BN + group * CW;
+            const bool half = CG == 2 && i.half >= 0;                    // a half tile's columns go round all groups too: half the slabs for each
+            const int slabs = half ? SLABS / 2 : SLABS, tile_col = group * slabs * 32;
+            const int row0 = i.m * 128 * CG + (int)rank * 128 + q * 32, col0 = i.n * BN + (half ? i.half * (BN / 2) : 0) + tile_col;
             if constexpr(EPI == EPI_SUM){
                 const int kb_begin = i.z * a.split_blocks, kb_end = min(k_blocks, kb_begin + a.split_blocks);
                 const int pieces = (kb_end - kb_begin + PIECE / KB - 1) / (PIECE / KB);
@@ -401,17 +419,14 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     const uint32_t b = acc & 1;
                     if(!tc::mbar_wait_bounded(acc_full + b, (acc >> 1) & 1, WAIT_LIMIT)){ ok = false; break; }
                     tc::fence_after_thread_sync();
-                    constexpr int AT_ONCE = 1;                           // registers: 64 sums and 32 of these
 #pragma unroll
-                    for(int j = 0; j < SLABS; j += AT_ONCE){
-                        uint32_t r[AT_ONCE][32];
-#pragma unroll
-                        for(int h = 0; h < AT_ONCE; h++) tc::tmem_ld_32x32(tmem + lanes + b * BN + group * CW + (j + h) * 32, r[h]);
+                    for(int j = 0; j < SLABS; j++){
+                        if(j >= slabs) break;
+                        uint32_t r[32];
+                        tc::tmem_ld_32x32(tmem + lanes + b * BN + tile_col + j * 32, r);
                         tc::tmem_wait_ld();
 #pragma unroll
-                        for(int h = 0; h < AT_ONCE; h++)
-#pragma unroll
-                            for(int c = 0; c < 32; c++) sum[j + h][c] += __uint_as_float(r[h][c]);
+                        for(int c = 0; c < 32; c++) sum[j][c] += __uint_as_float(r[c]);
                     }
                     tc::fence_before_thread_sync();
                     __syncwarp();
@@ -420,6 +435,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 if(!ok) break;
 #pragma unroll
                 for(int j = 0; j < SLABS; j++){
+                    if(j >= slabs) break;
                     uint32_t r[32];
 #pragma unroll
                     for(int c = 0; c < 32; c++) r[c] = __float_as_uint(sum[j][c]);
@@ -446,21 +462,21 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     }
                     break;
                 }
-                tc::tmem_ld_32x32(tmem + lanes + b * BN + group * CW, r);
+                tc::tmem_ld_32x32(tmem + lanes + b * BN + tile_col, r);
 #pragma unroll 1
-                for(int j = 0; j < SLABS; j++){
+                for(int j = 0; j < slabs; j++){
                     const int col = col0 + j * 32;
                     tc::tmem_wait_ld();
                     __syncwarp();                                        // the slab before has been read
                     slab_in(slab, r, lane);
-                    if(j + 1 < SLABS) tc::tmem_ld_32x32(tmem + lanes + b * BN + group * CW + (j + 1) * 32, r);
+                    if(j + 1 < slabs) tc::tmem_ld_32x32(tmem + lanes + b * BN + tile_col + (j + 1) * 32, r);
                     else tc::fence_before_thread_sync();
                     __syncwarp();
-                    if(j + 1 == SLABS && lane == 0) arrive_at_leader<CG>(acc_empty + b);
+                    if(j + 1 == slabs && lane == 0) arrive_at_leader<CG>(acc_empty + b);
                     if(row0 >= a.m || col >= a.n) continue;
                     if(!a.fast){ finish_slab_by_rows<T, EPI>(a, slab, row0, col, lane); continue; }
                     finish_whole_or_part<T, EPI>(a, slab, o, row0, col, lane);
-                    if(j + 1 < SLABS) fetch_slab<T, EPI>(o, a, row0, col + 32, lane);
+                    if(j + 1 < slabs) fetch_slab<T, EPI>(o, a, row0, col + 32, lane);
                 }
             }
         }
@@ -600,17 +616,21 @@ __global__ void __launch_bounds__(256) finish_kernel(FinishArgs f){
         }
 }
 
-// rows of 16-bit elements at any address -> rows that start on 16-byte boundaries, eight elements a thread
-__global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* src, long long ld, uint16_t* dst, long long ld_dst, long long rows, int cols){
+// Rows of 16-bit elements at any address -> rows that start on 16-byte boundaries, eight elements a thread; one operand or both
+struct AlignRows { const uint16_t* src; long long ld; uint16_t* dst; long long ld_dst, rows; int cols; };
+__global__ void __launch_bounds__(256) align_rows_kernel(AlignRows first, AlignRows second){
     after_predecessor();
-    const int chunks = (int)(ld_dst / 8);
-    const long long total = rows * chunks;
+    const long long chunks_1 = first.rows * (first.ld_dst / 8), total = chunks_1 + second.rows * (second.ld_dst / 8);
     for(long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll){
-        const long long r = i / chunks; const int c = (int)(i - r * chunks) * 8;
+        const bool one = i < chunks_1;
+        const AlignRows& o = one ? first : second;
+        const long long at = one ? i : i - chunks_1;
+        const int chunks = (int)(o.ld_dst / 8);
+        const long long r = at / chunks; const int c = (int)(at - r * chunks) * 8;
         union { uint4 v; uint16_t e[8]; } u;
 #pragma unroll
-        for(int j = 0; j < 8; j++) u.e[j] = c + j < cols ? src[r * ld + c + j] : (uint16_t)0;
-        *reinterpret_cast<uint4*>(dst + r * ld_dst + c) = u.v;
+        for(int j = 0; j < 8; j++) u.e[j] = c + j < o.cols ? o.src[r * o.ld + c + j] : (uint16_t)0;
+        *reinterpret_cast<uint4*>(o.dst + r * o.ld_dst + c) = u.v;
     }
 }
 
@@ -645,7 +665,7 @@ static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, l
 }
 
 struct TcPlan {
-    int cg, bn, m_tiles, n_tiles, splits, split_blocks, cluster_splits;
+    int cg, bn, m_tiles, n_tiles, splits, split_blocks, cluster_splits, whole_tiles;
     bool copy_a, copy_b, partial;
     long long ld_copy_a, ld_copy_b, ld_partial;
     size_t off_b, off_partial, off_sums, bytes;
@@ -668,7 +688,9 @@ static TcPlan plan_product(const Product& g, int epilogue){
             const int most = by_cluster ? (shares == 8 ? 15 : shares == 4 ? 33 : 74) : NUM_SMS / shares;     // clusters that are resident together
             if(shares > 1 && (tiles > most || k_blocks < 2 * shares)) break;
             const int blocks = (k_blocks - 1) / shares + 1;
-            const double cycles = (double)((tiles * shares - 1) / groups + 1) * (blocks * block + 1500.0) + (shares > 1 ? 2500.0 : 0.0);
+            const long long whole = tiles * shares / groups, rest = tiles * shares % groups;
+            const double rounds = whole + (rest == 0 ? 0.0 : cg == 2 && whole > 0 && 2 * rest <= groups ? 0.75 : 1.0);     // a half tile loads all of A
+            const double cycles = rounds * (blocks * block + 1500.0) + (shares == 1 ? 0.0 : by_cluster ? 2500.0 : 6000.0);      // the last: a launch and a pass over the partial sums
             if(best == 0.0 || cycles < best){
                 best = cycles;
                 p.cg = cg; p.bn = bn; p.m_tiles = (int)m_tiles; p.n_tiles = (int)n_tiles; p.split_blocks = blocks;
@@ -687,6 +709,8 @@ static TcPlan plan_product(const Product& g, int epilogue){
             p.splits = (k_blocks - 1) / p.split_blocks + 1;
         }
     }
+    const long long all = (long long)p.m_tiles * p.n_tiles * p.splits, last = all % (NUM_SMS / 2);
+    p.whole_tiles = (int)(p.cg == 2 && 2 * last <= NUM_SMS / 2 ? all - last : all);
     // operands that TMA cannot address are copied
     p.copy_a = !rows_aligned(g.a.p, g.a.ld, 2) && !(matrix_rows(g.a, g.m, g.k) <= 1 && reinterpret_cast<uintptr_t>(g.a.p) % 16 == 0);
     p.copy_b = !rows_aligned(g.b.p, g.b.ld, 2) && !(matrix_rows(g.b, g.n, g.k) <= 1 && reinterpret_cast<uintptr_t>(g.b.p) % 16 == 0);
@@ -704,13 +728,6 @@ static TcPlan plan_product(const Product& g, int epilogue){
     return p;
 }
 size_t product_tc_workspace_bytes(const Product& g, int epilogue){ return plan_product(g, epilogue).bytes; }
-
-static int align_rows(const Operand& o, long long rows, long long cols, void* dst, long long ld_dst, cudaStream_t s){
-    const long long blocks = (rows * (ld_dst / 8) + 255) / 256;
-    B200RL_CUDA_TRY(launch_after(align_rows_kernel, dim3((unsigned)(blocks < NUM_SMS * 16 ? blocks : NUM_SMS * 16)), dim3(256), 0, s, static_cast<const uint16_t*>(o.p), o.ld,
-                                 static_cast<uint16_t*>(dst), ld_dst, rows, (int)cols));
-    return B200RL_OK;
-}
 
 template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI>
 static int launch_tc(const CUtensorMap (&maps)[2], const TcArgs& a, cudaStream_t s){
@@ -737,7 +754,7 @@ static int launch_tc(const CUtensorMap (&maps)[2], const TcArgs& a, cudaStream_t
         groups[dev].store(most, std::memory_order_release);
     }
     // a tile that is shared has a cluster of its own; else as many CTAs (or pairs) as run at the same time take the tiles in turn
-    const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
+    const long long all = (long long)a.m_tiles * a.n_tiles * a.splits, tiles = 2 * all - a.whole_tiles;
     cfg.gridDim = (unsigned)(a.cluster_splits > 1 ? tiles * cluster : CG * (tiles < most ? tiles : most));
     cfg.numAttrs = 2;
     B200RL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], a));
@@ -761,13 +778,18 @@ static int product_tc_typed(const Product& g, int type, int epilogue, void* work
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     Operand A = g.a, B = g.b;
     int rc;
-    if(p.copy_a){
-        if((rc = align_rows(A, matrix_rows(A, g.m, g.k), matrix_cols(A, g.m, g.k), ws, p.ld_copy_a, s))) return rc;
-        A.p = ws; A.ld = p.ld_copy_a;
-    }
-    if(p.copy_b){
-        if((rc = align_rows(B, matrix_rows(B, g.n, g.k), matrix_cols(B, g.n, g.k), ws + p.off_b, p.ld_copy_b, s))) return rc;
-        B.p = ws + p.off_b; B.ld = p.ld_copy_b;
+    if(p.copy_a || p.copy_b){
+        AlignRows copies[2] = {};
+        int n = 0;
+        auto copy = [&](Operand& o, int r, void* dst, long long ld_dst){
+            copies[n++] = {static_cast<const uint16_t*>(o.p), o.ld, static_cast<uint16_t*>(dst), ld_dst, matrix_rows(o, r, g.k), (int)matrix_cols(o, r, g.k)};
+            o.p = dst; o.ld = ld_dst;
+        };
+        if(p.copy_a) copy(A, g.m, ws, p.ld_copy_a);
+        if(p.copy_b) copy(B, g.n, ws + p.off_b, p.ld_copy_b);
+        if(n == 1) copies[1] = {nullptr, 0, nullptr, 8, 0, 0};
+        const long long blocks = (copies[0].rows * (copies[0].ld_dst / 8) + copies[1].rows * (copies[1].ld_dst / 8) + 255) / 256;
+        B200RL_CUDA_TRY(launch_after(align_rows_kernel, dim3((unsigned)(blocks < NUM_SMS * 16 ? blocks : NUM_SMS * 16)), dim3(256), 0, s, copies[0], copies[1]));
     }
     float* partial = reinterpret_cast<float*>(ws + p.off_partial);
     TcArgs a{};
@@ -776,12 +798,14 @@ static int product_tc_typed(const Product& g, int type, int epilogue, void* work
     const uint32_t format = type == B200RL_TYPE_BFLOAT16 ? 1u : 0u;
     // fp32 sums, both operands of one type, their k_rows forms, N / 8, M / 16
     a.idesc = 1u << 4 | format << 7 | format << 10 | (A.k_rows ? 1u << 15 : 0u) | (B.k_rows ? 1u << 16 : 0u) | (uint32_t)(p.bn / 8) << 17 | (uint32_t)(128 * p.cg / 16) << 24;
+    a.idesc_half = (a.idesc & ~(0x3Fu << 17)) | (uint32_t)(p.bn / 16) << 17;
+    a.whole_tiles = p.whole_tiles;
     a.bias = g.bias; a.add = g.add; a.ld_add = g.ld_add; a.pre = g.pre; a.ld_pre = g.ld_pre; a.out = g.out; a.ld_out = g.ld_out;
     a.scale = g.scale; a.act = g.act; a.accumulate = g.accumulate;
     CUtensorMap maps[2] = {};
     const CUtensorMapDataType dt = type == B200RL_TYPE_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if((rc = make_map(&maps[0], dt, A.p, matrix_rows(A, g.m, g.k), matrix_cols(A, g.m, g.k), A.ld, A.k_rows ? 64 : 128))) return rc;
-    if((rc = make_map(&maps[1], dt, B.p, matrix_rows(B, g.n, g.k), matrix_cols(B, g.n, g.k), B.ld, B.k_rows ? 64 : p.bn / p.cg))) return rc;
+    if((rc = make_map(&maps[1], dt, B.p, matrix_rows(B, g.n, g.k), matrix_cols(B, g.n, g.k), B.ld, 64))) return rc;
     FinishArgs f{partial, p.ld_partial, p.ld_partial * (long long)g.m, p.splits, nullptr, a, g.row_sums};
     if(epilogue == EPI_SUM){
         TcArgs b = a;
