@@ -681,8 +681,8 @@ int b200rl_shuffle_rows(float* data, int ld, int n_rows, unsigned long long colu
 /* pre = x W^T + bias; y = residual + scale act(pre). type: bfloat16 or float16 (b200rl_dense_forward is the fp32 layer). W [output, input],
  * x [batch, input], bias fp32 [output] or NULL, residual [batch, output] or NULL (none added); pre [batch, output] or NULL receives the
  * pre-activations, which the backward pass needs for every activation but the identity. y may be residual itself (same pitch).
- * workspace: ..._workspace_bytes of the same operands (16-byte aligned; 0 bytes and NULL for most calls): split-k partial sums of small
- * batches, and copies of operands whose rows are not 16-byte aligned. Nothing in it is kept between calls. */
+ * workspace: ..._workspace_bytes of the same operands (16-byte aligned; 0 bytes and NULL for rows that start on 16-byte boundaries and for up to 32 rows): copies of
+ * operands whose rows the tensor cores' loads cannot address. Nothing in it is kept between calls. */
 size_t b200rl_dense_residual_forward_workspace_bytes(const void* W, int ldw, const void* x, int ldx, int batch, int input_dim, int output_dim);
 int b200rl_dense_residual_forward(int type, const void* W, int ldw, const float* bias, const void* x, int ldx, const void* residual, int ldr, float scale,
                                   void* pre, int ldpre, void* y, int ldy, int batch, int input_dim, int output_dim, int activation,
@@ -703,7 +703,7 @@ int b200rl_dense_residual_backward_input(int type, const void* W, int ldw, const
 
 /* d_W [output, input] (dense rows) = d_pre^T x and d_bias [output] = column sums of d_pre (either may be NULL), both fp32; accumulate != 0 adds onto
  * what they hold, 0 overwrites it. Every sum has a fixed order. The batch is summed in fp32 pieces of 512 rows, so that long batches lose nothing
- * to the tensor core's accumulator, which truncates. */
+ * to the tensor core's accumulator, which truncates. workspace: as above, and partial sums of long batches of small layers. */
 size_t b200rl_dense_residual_backward_weights_workspace_bytes(const void* x, int ldx, const void* d_pre, int ldd, const float* d_W, int batch, int input_dim, int output_dim);
 int b200rl_dense_residual_backward_weights(int type, const void* x, int ldx, const void* d_pre, int ldd, float* d_W, float* d_bias, int accumulate, int batch,
                                            int input_dim, int output_dim, void* workspace, size_t workspace_bytes, b200rl_stream_t stream);

@@ -3,27 +3,38 @@
 
 namespace b200rl {
 
+// Column sums (the bias gradient where the weights' is not asked for): 32 columns a CTA, 32 threads a column, each every 32nd row, then one after another in their order
 template <typename T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const T* d, long long ld, int rows, int cols, float* out, int accumulate){
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if(c >= cols) return;
+__global__ void __launch_bounds__(1024) column_sums_kernel(const T* d, long long ld, int rows, int cols, float* out, int accumulate){
+    __shared__ float shared[32][32];
+    after_predecessor();
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float v = 0.0f;
-    for(int r0 = 0; r0 < rows; r0 += 512){
-        float piece = 0.0f;
-        for(int r = r0; r < min(rows, r0 + 512); r++) piece += to_float(d[r * ld + c]);
-        v += piece;
-    }
+    if(c < cols)
+#pragma unroll 8
+        for(int r = slice; r < rows; r += 32) v += to_float(d[r * ld + c]);
+    shared[slice][lane] = v;
+    __syncthreads();
+    if(slice || c >= cols) return;
+#pragma unroll
+    for(int i = 1; i < 32; i++) v += shared[i][lane];
     out[c] = accumulate ? out[c] + v : v;
 }
 
-template <typename T, int ACT>
+// Bound by memory: two or three 16-bit elements each. N elements a thread, of one row; rows on 16-byte boundaries are taken eight elements at a time.
+template <typename T, int ACT, int N>
 __global__ void __launch_bounds__(256) backward_activation_kernel(const T* pre, long long ldp, const T* d_y, long long ldd, float scale, T* d_pre, long long ldo, int rows, int cols){
-    const size_t n = (size_t)rows * cols;
-    for(size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256){
-        const long long r = i / cols; const int c = (int)(i - r * cols);
-        float v = scale * to_float(d_y[r * ldd + c]);
-        if constexpr(ACT != B200RL_ACT_IDENTITY) v *= residual_d_activation<ACT>(to_float(pre[r * ldp + c]));
-        d_pre[r * ldo + c] = from_float<T>(v);
+    after_predecessor();
+    const int chunks = (cols - 1) / N + 1;
+    const long long total = (long long)rows * chunks;
+    for(long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll){
+        const long long r = i / chunks; const int c = (int)(i - r * chunks) * N;
+        float v[N], p[N];
+        load_elements(d_y + r * ldd + c, v);
+        if constexpr(ACT != B200RL_ACT_IDENTITY) load_elements(pre + r * ldp + c, p);
+#pragma unroll
+        for(int j = 0; j < N; j++){ v[j] *= scale; if constexpr(ACT != B200RL_ACT_IDENTITY) v[j] *= residual_d_activation<ACT>(p[j]); }
+        store_elements(d_pre + r * ldo + c, v);
     }
 }
 
@@ -98,12 +109,13 @@ int b200rl_dense_residual_backward_activation(int type, const void* pre, int ldp
     if(rows == 0) return B200RL_OK;
     if(!valid_matrix(d_y, ldd, rows, cols, 2) || !valid_matrix(d_pre, lddp, rows, cols, 2) ||
        (activation != B200RL_ACT_IDENTITY && !valid_matrix(pre, ldpre, rows, cols, 2))) return B200RL_ERR_INVALID_ARGUMENT;
-    const size_t blocks = ((size_t)rows * cols + 255) / 256;
-    const int grid = (int)(blocks < NUM_SMS * 8 ? blocks : NUM_SMS * 8);
-    B200RL_DISPATCH_16_BIT_TYPE(type, B200RL_DISPATCH_RESIDUAL_ACT(activation, (backward_activation_kernel<T, ACT><<<grid, 256, 0, (cudaStream_t)stream>>>(
-        static_cast<const T*>(pre), row_pitch(ldpre, rows, cols), static_cast<const T*>(d_y), row_pitch(ldd, rows, cols), scale, static_cast<T*>(d_pre),
-        row_pitch(lddp, rows, cols), rows, cols))))
-    B200RL_LAUNCH_CHECK("dense_residual_backward_activation");
+    const long long ldp = row_pitch(ldpre, rows, cols), lds = row_pitch(ldd, rows, cols), ldo = row_pitch(lddp, rows, cols);
+    const bool vector = cols % 8 == 0 && rows_aligned(d_y, lds, 2) && rows_aligned(d_pre, ldo, 2) && (activation == B200RL_ACT_IDENTITY || rows_aligned(pre, ldp, 2));
+    const long long blocks = ((long long)rows * (vector ? cols / 8 : cols) + 255) / 256;
+    const dim3 grid((unsigned)(blocks < NUM_SMS * 8 ? blocks : NUM_SMS * 8));
+    B200RL_DISPATCH_16_BIT_TYPE(type, B200RL_DISPATCH_RESIDUAL_ACT(activation,
+        B200RL_CUDA_TRY(launch_after(vector ? backward_activation_kernel<T, ACT, 8> : backward_activation_kernel<T, ACT, 1>, grid, dim3(256), 0, (cudaStream_t)stream,
+                                     static_cast<const T*>(pre), ldp, static_cast<const T*>(d_y), lds, scale, static_cast<T*>(d_pre), ldo, rows, cols))))
     return B200RL_OK;
 }
 
@@ -145,9 +157,8 @@ int b200rl_dense_residual_backward_weights(int type, const void* x, int ldx, con
         return product_tc(g, type, EPI_SUM, workspace, (cudaStream_t)stream);
     }
     if(d_bias){
-        B200RL_DISPATCH_16_BIT_TYPE(type, column_sums_kernel<T><<<(output_dim + 255) / 256, 256, 0, (cudaStream_t)stream>>>(static_cast<const T*>(d_pre),
-            row_pitch(ldd, batch, output_dim), batch, output_dim, d_bias, accumulate))
-        B200RL_LAUNCH_CHECK("dense_residual bias gradient");
+        B200RL_DISPATCH_16_BIT_TYPE(type, B200RL_CUDA_TRY(launch_after(column_sums_kernel<T>, dim3((output_dim - 1) / 32 + 1), dim3(1024), 0, (cudaStream_t)stream,
+                                                                        static_cast<const T*>(d_pre), row_pitch(ldd, batch, output_dim), batch, output_dim, d_bias, accumulate)))
     }
     return B200RL_OK;
 }

@@ -6,6 +6,7 @@
 // Measured (bfloat16, 1024 -> 4096): 1 row 3.1 us, 16 rows 3.3 us, 32 rows 4.8 us (64 would be 7.5), where W's 8.4 MB take 1.3 us at the rate of memory and a launch about 2; the
 // tensor-memory kernel takes 8.5 us.
 #include "product.cuh"
+#include <limits.h>
 
 namespace b200rl {
 
@@ -53,7 +54,7 @@ __global__ void __launch_bounds__(256) product_rows_kernel(RowsArgs a){
 #pragma unroll
     for(int j = 0; j < NT; j++) x[j] = static_cast<const T*>(a.x) + min(j * 8 + g, a.m - 1) * a.ldx;
     float acc[NT][4] = {};
-    const int blocks = (a.k + 31) / 32;
+    const int blocks = (a.k - 1) / 32 + 1;
     for(int kb = warp; kb < blocks; kb += 8 * AHEAD){
         uint4 wv[AHEAD][2], xv[AHEAD][NT];
 #pragma unroll
@@ -100,7 +101,7 @@ static int launch_rows(const RowsArgs& a, cudaStream_t s){
     return B200RL_OK;
 }
 
-bool product_rows_takes(const Product& g){ return g.m <= 32 && !g.a.k_rows && !g.b.k_rows; }
+bool product_rows_takes(const Product& g){ return g.m <= 32 && !g.a.k_rows && !g.b.k_rows && g.n <= INT_MAX - 1024 && g.k <= INT_MAX - 1024; }
 int product_rows(const Product& g, int type, cudaStream_t s){
     const RowsArgs a{g.a.p, g.a.ld, g.b.p, g.b.ld, g.m, g.n, g.k, g.bias, g.add, g.ld_add, g.pre, g.ld_pre, g.out, g.ld_out, g.scale, g.act};
     const bool aligned = (g.m == 1 ? reinterpret_cast<uintptr_t>(g.a.p) % 16 == 0 : rows_aligned(g.a.p, g.a.ld, 2)) &&

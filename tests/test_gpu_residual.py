@@ -204,6 +204,126 @@ def test_dense_values_that_are_not_finite_stay_in_their_row(lib):
         assert torch.equal(y[rows], clean[rows]) and not torch.isfinite(y[3]).any() and torch.isnan(y[5]).all()
 
 
+@pytest.mark.parametrize("layout", [(16, 8), (5, 3)])
+@pytest.mark.parametrize("B", [9, 140])
+def test_dense_backward_reads_only_its_views(lib, B, layout):
+    """NaN behind and in front of every operand's rows, and in the rows behind the last, reach nothing."""
+    g, (pad, offset), I, O = seeded(9), layout, 72, 50
+
+    def island(rows, cols, std=1.0):
+        t = torch.full((rows + 3, cols + pad), float("nan"), device="cuda", dtype=BF16)
+        t[:rows, offset:offset + cols] = (torch.randn(rows, cols, device="cuda", generator=g) * std).to(BF16)
+        return t[:rows, offset:offset + cols]
+
+    W, x, d, a, p = island(O, I), island(B, I), island(B, O), island(B, I), island(B, I)
+    got = lib.dense_residual_backward(W, x, d, add=a, pre_in=p, act_in="silu")
+    want = lib.dense_residual_backward(*(t.contiguous() for t in (W, x, d)), add=a.contiguous(), pre_in=p.contiguous(), act_in="silu")
+    for u, v in zip(got, want):
+        assert torch.isfinite(u).all() and torch.equal(u, v)
+    pre, y = lib.dense_residual_forward(W, x, "silu", residual=island(B, O), want_pre=True)
+    assert torch.isfinite(y).all() and torch.isfinite(pre).all()
+
+
+def test_dense_weight_gradients_at_any_address_and_alone(lib):
+    """Slices of a parameter arena at odd offsets; through the C entry point one gradient without the other."""
+    B, I, O = 700, 90, 77
+    g, x, _ = dense_inputs(B, I, O, BF16, 0, 0, 12)
+    d = table(B, O, BF16, g, std=0.25)[0]
+    W = x.new_zeros(O, I)
+    d_W, d_b, _ = lib.dense_residual_backward(W, x, d, want_d_in=False)
+    arena = torch.full((O * I + O + 8,), 5.0, device="cuda")
+    a_W, a_b = arena[3:3 + O * I].view(O, I), arena[3 + O * I:3 + O * I + O]
+    a_W.zero_()
+    a_b.zero_()
+    lib.dense_residual_backward(W, x, d, d_W=a_W, d_bias=a_b, want_d_in=False)
+    assert torch.equal(a_W, d_W) and torch.equal(a_b, d_b) and (arena[:3] == 5).all() and (arena[3 + O * I + O:] == 5).all()
+    L, st = lib.lib(), torch.cuda.current_stream().cuda_stream
+    n = L.b200rl_dense_residual_backward_weights_workspace_bytes(x.data_ptr(), I, d.data_ptr(), O, a_W.data_ptr(), B, I, O)
+    ws = torch.empty(max(n, 16), device="cuda", dtype=torch.uint8)
+    only_W, only_b = torch.empty_like(d_W), torch.ones_like(d_b)
+    assert L.b200rl_dense_residual_backward_weights(1, x.data_ptr(), I, d.data_ptr(), O, only_W.data_ptr(), None, 0, B, I, O, ws.data_ptr(), n, st) == 0
+    assert L.b200rl_dense_residual_backward_weights(1, None, 0, d.data_ptr(), O, None, only_b.data_ptr(), 1, B, I, O, None, 0, st) == 0
+    assert torch.equal(only_W, d_W)
+    want = d.double().sum(0)
+    assert_within(only_b, 1 + want, (B + 3) * U32 * (1 + d.double().abs().sum(0)), "d_bias")
+
+
+def test_offsets_beyond_32_bits(lib):
+    """Rows 40,000 elements apart: the last ones lie more than 2^31 elements behind the first."""
+    R, ld, I, O = 66000, 40000, 64, 40
+    assert R * ld > 2 ** 31
+    big = torch.empty(R, ld, device="cuda", dtype=BF16)
+    x, y, r = big[:, :I], big[:, 1000:1000 + O], big[:, 2000:2000 + O]
+    g = seeded(13)
+    x.copy_(torch.randn(R, I, device="cuda", generator=g))
+    r.copy_(torch.randn(R, O, device="cuda", generator=g))
+    W = torch.randn(O, I, device="cuda", generator=g).to(BF16)
+    lib.dense_residual_forward(W, x, "relu", residual=r, y=y)
+    assert torch.equal(y, lib.dense_residual_forward(W, x.contiguous(), "relu", residual=r.contiguous())[1])
+    d_W, d_b, d_in = lib.dense_residual_backward(W, x, r, add=x, d_in=big[:, 3000:3000 + I])
+    want = lib.dense_residual_backward(W, x.contiguous(), r.contiguous(), add=x.contiguous())
+    assert all(torch.equal(a, b) for a, b in zip((d_W, d_b, d_in), want))
+    out, normed = lib.norm_residual_forward(y, r, post="rms", pre="layer", out=big[:, 4000:4000 + O], normed=big[:, 5000:5000 + O])
+    want = lib.norm_residual_forward(y.contiguous(), r.contiguous(), post="rms", pre="layer")
+    assert torch.equal(out, want[0]) and torch.equal(normed, want[1])
+    got = lib.norm_residual_backward(y, out, r, normed, post="rms", pre="layer")
+    want = lib.norm_residual_backward(y.contiguous(), out.contiguous(), r.contiguous(), normed.contiguous(), post="rms", pre="layer")
+    assert torch.equal(got["d_branch"], want["d_branch"]) and torch.equal(got["d_residual"], want["d_residual"])
+    assert torch.equal(lib.dropout(x, 0.3, 5, y=big[:, 6000:6000 + I]), lib.dropout(x.contiguous(), 0.3, 5))
+
+
+def test_calls_on_two_streams_at_once(lib):
+    """Nothing is shared between calls: products that split k and share workspaces' sizes run on two streams and give what each gives alone."""
+    jobs = []
+    for n, (B, I, O) in enumerate([(3000, 70, 66), (2900, 66, 70)]):
+        g, x, W = dense_inputs(B, I, O, BF16, 0, 0, n)
+        d = table(B, O, BF16, g, std=0.25)[0]
+        jobs.append((W, x, d, [t.clone() for t in lib.dense_residual_backward(W, x, d)]))
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in jobs], [[], []]
+    for _ in range(20):
+        for s, (W, x, d, _), out in zip(streams, jobs, results):
+            with torch.cuda.stream(s):
+                out.append(lib.dense_residual_backward(W, x, d))
+    torch.cuda.synchronize()
+    for (_, _, _, want), out in zip(jobs, results):
+        assert all(torch.equal(a, b) for got in out for a, b in zip(got, want))
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, {root!r})
+import __graft_entry__ as entry
+lib = entry.load_package()
+import torch
+T = torch.bfloat16
+x, W, d = torch.ones(300, 64, device="cuda", dtype=T), torch.ones(48, 64, device="cuda", dtype=T), torch.ones(300, 48, device="cuda", dtype=T)
+w = torch.ones(64, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = lib.dense_residual_forward(W, x, "identity")[1]
+    one = lib.dense_residual_forward(W, x[:1], "identity")[1]
+    d_W, d_b, d_in = lib.dense_residual_backward(W, x, d)
+    out, normed = lib.norm_residual_forward(x, x, post="rms", post_weight=w, pre="layer", pre_weight=w)
+    g = lib.norm_residual_backward(x, out, x, normed, post="rms", post_weight=w, pre="layer", pre_weight=w)
+    drop = lib.dropout(x, 0.5, 1)
+graph.replay()
+torch.cuda.synchronize()
+assert (y == 64).all() and (one == 64).all() and (d_W == 300).all() and (d_b == 300).all() and (d_in == 48).all()
+assert torch.isfinite(g["d_branch"]).all() and ((drop == 0) | (drop == 2)).all()
+print("captured first")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured(lib):
+    import subprocess
+    import sys
+    from conftest import ROOT
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=ROOT)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured first" in done.stdout, done.stdout + done.stderr
+
+
 # ---- norms -------------------------------------------------------------------------------------------------------------------------------------
 NORM_SIZES = [(1, 1), (1, 4096), (3, 5), (7, 64), (50, 257), (33, 512), (130, 777), (64, 1024), (20, 2048), (9, 2049), (300, 100), (5, 4097), (4, 8192), (700, 33), (2500, 16)]
 

@@ -46,6 +46,29 @@ def test_dense_entry_points_refuse(lib):
     assert backward_activation(out=None) == 1 and backward_activation(ld=7) == 1 and backward_activation(cols=0) == 1 and backward_activation(rows=0) == 0
 
 
+def test_workspaces_are_asked_for_and_checked(lib):
+    """Rows that start on 16-byte boundaries need none; rows that do not are copied, and a call without the room for it is refused."""
+    L, p = lib.lib(), ADDRESS
+    size = L.b200rl_dense_residual_forward_workspace_bytes
+    assert size(p, 64, p, 64, 500, 64, 64) == 0 and size(p, 65, p, 65, 20, 64, 64) == 0
+    n = size(p, 65, p, 64, 500, 64, 64)
+    assert n >= 64 * 64 * 2 and size(p, 64, p + 2, 64, 500, 64, 64) >= 500 * 64 * 2 and size(p, 65, p, 65, 0, 64, 64) == 0
+
+    def forward(ws, n):
+        return L.b200rl_dense_residual_forward(1, p, 65, None, p, 64, None, 0, 1.0, None, 0, p, 64, 500, 64, 64, 0, ws, n, None)
+
+    assert forward(None, 0) == 1 and forward(p, n - 1) == 1 and forward(p + 8, n) == 1
+    size = L.b200rl_dense_residual_backward_weights_workspace_bytes
+    assert size(p, 4096, p, 4096, p, 4096, 4096, 4096) == 0 and size(p, 64, p, 64, None, 100000, 64, 64) == 0
+    n = size(p, 64, p, 64, p, 100000, 64, 64)
+    assert n > 0
+    assert L.b200rl_dense_residual_backward_weights(1, p, 64, p, 64, p, None, 0, 100000, 64, 64, p, n - 256, None) == 1
+    assert L.b200rl_dense_residual_backward_input_workspace_bytes(p, 63, p, 64, 100, 63, 64) >= 64 * 64 * 2
+    # sizes that no memory holds are refused, not computed with
+    top = 2 ** 31 - 1
+    assert L.b200rl_dense_residual_forward(1, p, top, None, p, top, None, 0, 1.0, None, 0, p, top, top, top, top, 0, p, 1 << 62, None) == 2
+
+
 def test_norm_entry_points_refuse(lib):
     L = lib.lib()
     p = ADDRESS
