@@ -74,6 +74,15 @@ template <int CG> __device__ __forceinline__ void load_box(void* smem, const CUt
         asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                      :: "r"(tc::smem_u32(smem)), "l"(map), "r"(leader_address(bar)), "r"(x), "r"(y) : "memory");
 }
+// One lane of a converged warp. The loops that issue loads and MMAs are run by whole warps and only the instructions themselves by this lane: their operands then stay in uniform
+// registers. Run by a single thread, the same loop takes 650 cycles for a stage whatever the tile, more than the MMAs of the largest (512).
+__device__ __forceinline__ bool elected(){
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+// a bounded wait of a whole warp, which goes on or gives up together
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity){ return __all_sync(0xffffffffu, tc::mbar_wait_bounded(bar, parity, WAIT_LIMIT)); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map){ asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory"); }
 template <int CG> __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate){
     if constexpr(CG == 1) tc::mma_f16_ss(d, a, b, idesc, accumulate);
@@ -301,7 +310,6 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     uint64_t* full = reinterpret_cast<uint64_t*>(staging + EPI_WARPS * STAGING);
     uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + 2;
     uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
     float* sum_buffer = reinterpret_cast<float*>(slot + 4);                  // [2][SUM_COLUMNS]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;                 // in a pair
@@ -311,7 +319,6 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         for(int s = 0; s < STAGES; s++){ tc::mbar_init(full + s, 1); tc::mbar_init(empty + s, 1); }
         for(int b = 0; b < 2; b++){ tc::mbar_init(acc_full + b, 1); tc::mbar_init(acc_empty + b, CG * 4 * GROUPS); }
         tc::fence_mbar_init();
-        *abort_flag = 0;
     }
     if(warp == 2) tensor_memory_alloc<CG>(slot, 2 * BN);
     tc::fence_before_thread_sync();
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
 
     if(warp < 4){
         tc::setmaxnreg_dec<64>();
-        if(warp == 0 && lane == 0){
+        if(warp == 0){
             uint32_t it = 0;
             bool ok = true;
             for(int t = first_tile; t < tiles && ok; t += tile_step){
@@ -336,30 +343,33 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 const int part = i.z + share, kb_end = min(k_blocks, (part + 1) * a.split_blocks);
                 for(int kb = part * a.split_blocks; kb < kb_end; kb++, it++){
                     const uint32_t s = it % STAGES, phase = (it / STAGES) & 1;
-                    if(!tc::mbar_wait_bounded(empty + s, phase ^ 1, WAIT_LIMIT) || *abort_flag){ ok = false; break; }
+                    if(!warp_wait(empty + s, phase ^ 1)){ ok = false; break; }
                     uint8_t* stage = base + s * STAGE;
-                    if(rank == 0) arrive_expect(full + s, CG * bytes);
-                    if constexpr(A_ROWS){
-                        load_box<CG>(stage, &map_a, m0, kb * KB, full + s);
-                        load_box<CG>(stage + 8192, &map_a, m0 + 64, kb * KB, full + s);
-                    }
-                    else load_box<CG>(stage, &map_a, kb * KB, m0, full + s);
+                    if(elected()){
+                        if(rank == 0) arrive_expect(full + s, CG * bytes);
+                        if constexpr(A_ROWS){
+                            load_box<CG>(stage, &map_a, m0, kb * KB, full + s);
+                            load_box<CG>(stage + 8192, &map_a, m0 + 64, kb * KB, full + s);
+                        }
+                        else load_box<CG>(stage, &map_a, kb * KB, m0, full + s);
 #pragma unroll
-                    for(int j = 0; j < BN / CG / 64; j++){                // boxes of 64 rows of B either way
-                        if(j >= BN / CG / 128 && half) break;
-                        if constexpr(B_ROWS) load_box<CG>(stage + A_BYTES + j * 8192, &map_b, n0 + 64 * j, kb * KB, full + s);
-                        else load_box<CG>(stage + A_BYTES + j * 8192, &map_b, kb * KB, n0 + 64 * j, full + s);
+                        for(int j = 0; j < BN / CG / 64; j++){                // boxes of 64 rows of B either way
+                            if(j >= BN / CG / 128 && half) break;
+                            if constexpr(B_ROWS) load_box<CG>(stage + A_BYTES + j * 8192, &map_b, n0 + 64 * j, kb * KB, full + s);
+                            else load_box<CG>(stage + A_BYTES + j * 8192, &map_b, kb * KB, n0 + 64 * j, full + s);
+                        }
                     }
+                    __syncwarp();
                 }
             }
             // no CTA leaves while its copies or its peer's signals are under way: the last use of every stage has been released
             for(uint32_t s = 0; s < STAGES && s < it; s++){
                 const uint32_t last = (it - 1 - s) / STAGES * STAGES + s;         // the last step of this stage
-                if(!tc::mbar_wait_bounded(empty + s, (last / STAGES) & 1, WAIT_LIMIT)) ok = false;
+                if(!warp_wait(empty + s, (last / STAGES) & 1)) ok = false;
             }
-            if(!ok){ *abort_flag = 1; g_product_tc_error = 1; }
+            if(!ok) g_product_tc_error = 1;
         }
-        else if(warp == 1 && lane == 0 && rank == 0){
+        else if(warp == 1 && rank == 0){
             uint32_t it = 0, acc = 0;
             bool ok = true;
             for(int t = first_tile; t < tiles && ok; t += tile_step){
@@ -370,26 +380,29 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 for(int kb0 = part * a.split_blocks; kb0 < kb_end && ok; acc++){
                     const int piece_end = EPI == EPI_SUM ? min(kb_end, kb0 + PIECE / KB) : kb_end;
                     const uint32_t b = acc & 1, d = tmem + b * BN;
-                    if(!tc::mbar_wait_bounded(acc_empty + b, ((acc >> 1) & 1) ^ 1, WAIT_LIMIT)){ ok = false; break; }
+                    if(!warp_wait(acc_empty + b, ((acc >> 1) & 1) ^ 1)){ ok = false; break; }
                     tc::fence_after_thread_sync();
                     for(int kb = kb0; kb < piece_end; kb++, it++){
                         const uint32_t s = it % STAGES;
-                        if(!tc::mbar_wait_bounded(full + s, (it / STAGES) & 1, WAIT_LIMIT) || *abort_flag){ ok = false; break; }
+                        if(!warp_wait(full + s, (it / STAGES) & 1)){ ok = false; break; }
                         tc::fence_after_thread_sync();
                         const uint32_t stage = tc::smem_u32(base + s * STAGE);
                         const uint64_t da = A_ROWS ? make_desc_rows_sw128(stage) : tc::make_desc_kmajor_sw128(stage);
                         const uint64_t db = B_ROWS ? make_desc_rows_sw128(stage + A_BYTES) : tc::make_desc_kmajor_sw128(stage + A_BYTES);
+                        if(elected()){
 #pragma unroll
-                        for(int ks = 0; ks < KB / 16; ks++)
-                            mma<CG>(d, da + (uint64_t)(ks * (A_ROWS ? 128 : 2)), db + (uint64_t)(ks * (B_ROWS ? 128 : 2)), idesc, (kb > kb0 || ks) ? 1u : 0u);
-                        commit<CG>(empty + s);
+                            for(int ks = 0; ks < KB / 16; ks++)
+                                mma<CG>(d, da + (uint64_t)(ks * (A_ROWS ? 128 : 2)), db + (uint64_t)(ks * (B_ROWS ? 128 : 2)), idesc, (kb > kb0 || ks) ? 1u : 0u);
+                            commit<CG>(empty + s);
+                            if(kb + 1 == piece_end) commit<CG>(acc_full + b);
+                        }
+                        __syncwarp();
                     }
                     if(!ok) break;
-                    commit<CG>(acc_full + b);
                     kb0 = piece_end;
                 }
             }
-            if(!ok){ *abort_flag = 1; g_product_tc_error = 1; }
+            if(!ok) g_product_tc_error = 1;
         }
         else if(EPI == EPI_SUM && warp >= 2 && a.sums) sum_rows<T>(a, sum_buffer, tid - 64, warp - 2, lane);
         __syncwarp();
@@ -417,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     for(int c = 0; c < 32; c++) sum[j][c] = 0.0f;
                 for(int p = 0; p < pieces; p++, acc++){
                     const uint32_t b = acc & 1;
-                    if(!tc::mbar_wait_bounded(acc_full + b, (acc >> 1) & 1, WAIT_LIMIT)){ ok = false; break; }
+                    if(!warp_wait(acc_full + b, (acc >> 1) & 1)){ ok = false; break; }
                     tc::fence_after_thread_sync();
 #pragma unroll
                     for(int j = 0; j < SLABS; j++){
@@ -450,7 +463,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 acc++;
                 SlabOperands o;
                 if(a.fast && sharers == 1) fetch_slab<T, EPI>(o, a, row0, col0, lane);
-                if(!tc::mbar_wait_bounded(acc_full + b, phase, WAIT_LIMIT)){ ok = false; break; }
+                if(!warp_wait(acc_full + b, phase)){ ok = false; break; }
                 tc::fence_after_thread_sync();
                 uint32_t r[32];
                 if(sharers > 1){                                         // one tile a cluster: its sums go where the operands were
@@ -480,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 }
             }
         }
-        if(!ok){ *abort_flag = 1; g_product_tc_error = 1; }
+        if(!ok) g_product_tc_error = 1;
         __syncwarp();
         if constexpr(CG == 1 && EPI != EPI_SUM) if(sharers > 1){
             // every CTA's sums are in place; each takes every so many-th slab, adds up the shares in their order and finishes it
