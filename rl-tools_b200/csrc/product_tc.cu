@@ -63,7 +63,8 @@ __device__ __forceinline__ uint32_t peer_address(const void* p, uint32_t rank){ 
 __device__ __forceinline__ void arrive_expect(uint64_t* bar, uint32_t bytes){ asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(tc::smem_u32(bar)), "r"(bytes) : "memory"); }
 template <int CG> __device__ __forceinline__ void arrive_at_leader(uint64_t* bar){
     if constexpr(CG == 1) tc::mbar_arrive(bar);
-    else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(leader_address(bar)) : "memory");
+    // what it hands over is tensor memory that has been read (ordered by the fence in front of it), so no store of this warp has to be waited for, as a release to the cluster would
+    else asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(leader_address(bar)) : "memory");
 }
 // a box of a matrix into this CTA's shared memory; its bytes count at the leader's barrier
 template <int CG> __device__ __forceinline__ void load_box(void* smem, const CUtensorMap* map, int x, int y, uint64_t* bar){
@@ -138,7 +139,7 @@ template <typename T> __device__ __forceinline__ void unpack_chunk(float (&f)[8]
 #pragma unroll
     for(int e = 0; e < 4; e++){ const float2 p = unpack<T>(u[e]); f[2 * e] = p.x; f[2 * e + 1] = p.y; }
 }
-template <typename T> __device__ __forceinline__ uint4 pack_chunk(const float (&v)[8]){ return make_uint4(pack<T>(v[0], v[1]), pack<T>(v[2], v[3]), pack<T>(v[4], v[5]), pack<T>(v[6], v[7])); }
+template <typename T> __device__ __forceinline__ uint4 pack_pairs(const float2 (&v)[4]){ return make_uint4(pack<T>(v[0].x, v[0].y), pack<T>(v[1].x, v[1].y), pack<T>(v[2].x, v[2].y), pack<T>(v[3].x, v[3].y)); }
 // eight consecutive elements at p (16-byte aligned), of which `count` exist
 template <typename T> __device__ __forceinline__ uint4 load_chunk(const T* p, int count){
     if(count >= 8) return *reinterpret_cast<const uint4*>(p);
@@ -162,13 +163,21 @@ template <typename T> __device__ __forceinline__ void store_chunk(T* p, const ui
 // covers whole sectors. 16-byte piece c of row r lies at piece c ^ (r % 8): neither direction has bank conflicts. Measured against outputs by TMA: those wait in the TMA unit's queue
 // behind up to five stages of operand loads, 2,500 cycles a slab, and a warp has no third buffer (16384 x 4096 x 4096 with a residual 470 us).
 __device__ __forceinline__ void slab_in(uint8_t* slab, const uint32_t (&r)[32], int lane){
+    const uint32_t row = tc::smem_u32(slab) + lane * 128 + ((lane & 7) << 4);        // piece 0; the others differ from it in bits 4 to 6
 #pragma unroll
-    for(int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(slab + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+    for(int c = 0; c < 8; c++)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(row ^ (c << 4)), "r"(r[4 * c]), "r"(r[4 * c + 1]), "r"(r[4 * c + 2]), "r"(r[4 * c + 3]) : "memory");
+}
+__device__ __forceinline__ float4 slab_load(uint32_t address){
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
+    return v;
 }
 __device__ __forceinline__ float4 slab_out(const uint8_t* slab, int row, int piece){ return *reinterpret_cast<const float4*>(slab + row * 128 + ((piece ^ (row & 7)) << 4)); }
 __device__ __forceinline__ float slab_element(const uint8_t* slab, int row, int column){ return *reinterpret_cast<const float*>(slab + row * 128 + (((column >> 2) ^ (row & 7)) << 4) + (column & 3) * 4); }
 
-// The operands of a slab's epilogue that lie in memory, 16-bit rows on 16-byte boundaries: a lane has eight columns of every eighth row. WHOLE: all of the slab is inside the matrix.
+// The operands of a slab's epilogue that lie in memory, 16-bit rows on 16-byte boundaries: a lane has eight columns (8 (lane % 4) on) of every eighth row, so that neighbours share a row's
+// sectors. WHOLE: all of the slab is inside the matrix.
 struct SlabOperands { uint4 add[4], pre[4]; };
 template <typename T> __device__ __forceinline__ void fetch_chunks(uint4 (&raw)[4], const T* p, long long ld, int rows, int count){
     if(rows >= 32 && count >= 8)
@@ -186,44 +195,47 @@ template <typename T, int EPI> __device__ __forceinline__ void fetch_slab(SlabOp
 template <typename T, int EPI, int ACT, bool WHOLE>
 __device__ __forceinline__ void finish_slab(const TcArgs& a, const uint8_t* slab, const SlabOperands& o, const float (&bias)[8], int row0, int col0, int lane){
     const int col = col0 + 8 * (lane & 3), row = row0 + (lane >> 2), count = a.n - col, rows = a.m - row;
+    const uint32_t from = tc::smem_u32(slab) + (lane >> 2) * 128 + (((2 * (lane & 3)) ^ (lane >> 2)) << 4);
     T* out = static_cast<T*>(a.out) + (long long)row * a.ld_out + col;
     T* pre = EPI == EPI_FORWARD && a.pre ? static_cast<T*>(a.pre) + (long long)row * a.ld_pre + col : nullptr;
+    const float2 scale = both(a.scale);
 #pragma unroll
     for(int i = 0; i < 4; i++, out += 8 * a.ld_out){
-        const float4 lo = slab_out(slab, 8 * i + (lane >> 2), 2 * (lane & 3)), hi = slab_out(slab, 8 * i + (lane >> 2), 2 * (lane & 3) + 1);
-        float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}, add[8];
+        const float4 lo = slab_load(from + i * 1024), hi = slab_load((from ^ 16) + i * 1024);
+        float2 v[4] = {make_float2(lo.x, lo.y), make_float2(lo.z, lo.w), make_float2(hi.x, hi.y), make_float2(hi.z, hi.w)};
+        float add[8];
         const bool there = WHOLE || (8 * i < rows && count > 0);
         const int elements = WHOLE ? 8 : count;
         if constexpr(EPI == EPI_FORWARD){
             if(a.bias)
 #pragma unroll
-                for(int c = 0; c < 8; c++) v[c] += bias[c];
+                for(int c = 0; c < 4; c++) v[c] = add2(v[c], make_float2(bias[2 * c], bias[2 * c + 1]));
             if(pre){
-                if(there) store_chunk(pre, pack_chunk<T>(v), elements);
+                if(there) store_chunk(pre, pack_pairs<T>(v), elements);
                 pre += 8 * a.ld_pre;
             }
-            activate8<ACT>(v);
+            activate_pairs<ACT>(v);
             if(a.add){
                 unpack_chunk<T>(add, o.add[i]);
 #pragma unroll
-                for(int c = 0; c < 8; c++) v[c] = fmaf(a.scale, v[c], add[c]);
+                for(int c = 0; c < 4; c++) v[c] = fma2(v[c], scale, make_float2(add[2 * c], add[2 * c + 1]));
             }
             else
 #pragma unroll
-                for(int c = 0; c < 8; c++) v[c] *= a.scale;
+                for(int c = 0; c < 4; c++) v[c] = mul2(v[c], scale);
         }
         else{
             if(a.add){
                 unpack_chunk<T>(add, o.add[i]);
 #pragma unroll
-                for(int c = 0; c < 8; c++) v[c] += add[c];
+                for(int c = 0; c < 4; c++) v[c] = add2(v[c], make_float2(add[2 * c], add[2 * c + 1]));
             }
             if constexpr(ACT != B200RL_ACT_IDENTITY){
                 unpack_chunk<T>(add, o.pre[i]);
-                times_slope8<ACT>(v, add);
+                times_slope_pairs<ACT>(v, add);
             }
         }
-        if(there) store_chunk(out, pack_chunk<T>(v), elements);
+        if(there) store_chunk(out, pack_pairs<T>(v), elements);
     }
 }
 template <typename T, int EPI> __device__ __forceinline__ void finish_whole_or_part(const TcArgs& a, const uint8_t* slab, const SlabOperands& o, int row0, int col, int lane){

@@ -125,6 +125,24 @@ template <int ACT> __device__ __forceinline__ void times_slope8(float (&v)[8], c
 #pragma unroll
         for(int c = 0; c < 8; c++) v[c] *= residual_d_activation<ACT>(at[c]);
 }
+template <int ACT> __device__ __forceinline__ void activate_pairs(float2 (&v)[4]){
+#pragma unroll
+    for(int c = 0; c < 4; c++){
+        if constexpr(ACT == B200RL_ACT_GELU) v[c] = mul2(v[c], normal_pair(v[c]).phi);
+        else v[c] = make_float2(residual_activation<ACT>(v[c].x), residual_activation<ACT>(v[c].y));
+    }
+}
+template <int ACT> __device__ __forceinline__ void times_slope_pairs(float2 (&v)[4], const float (&at)[8]){
+#pragma unroll
+    for(int c = 0; c < 4; c++){
+        const float2 x = make_float2(at[2 * c], at[2 * c + 1]);
+        if constexpr(ACT == B200RL_ACT_GELU){
+            const NormalPair n = normal_pair(x);
+            v[c] = mul2(v[c], fma2(mul2(x, both(0.39894228040143268f)), n.density, n.phi));
+        }
+        else v[c] = mul2(v[c], make_float2(residual_d_activation<ACT>(x.x), residual_d_activation<ACT>(x.y)));
+    }
+}
 #define B200RL_DISPATCH_RESIDUAL_ACT(act, ...) \
     switch(act){ \
         case B200RL_ACT_GELU: { constexpr int ACT = B200RL_ACT_GELU; __VA_ARGS__; break; } \
