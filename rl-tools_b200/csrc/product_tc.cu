@@ -707,7 +707,9 @@ static TcPlan plan_product(const Product& g, int epilogue){
     TcPlan p{};
     const int k_blocks = (g.k - 1) / KB + 1;
     // Shape of the tiles and shares of k, by the cycles that a CTA needs: for a block of 64 k the bytes of its stage at the 48 a cycle that L2 gives a multiprocessor when all ask
-    // (measured; the MMAs take 128 to 512), for a tile 1,500 until its sums are out, for a shared tile 2,500 more. Sharing a tile needs a CTA for each share at the same time.
+    // (measured; the MMAs take 128 to 512), for a tile 1,500 until its sums are out, for a shared tile 1,500 and 1,000 a share more. Sharing a tile needs a CTA for each share at the
+    // same time. us by tiles of 64 / 128 / 256 columns (* the rule's choice): 1024 x 1024 x 1024 7.8* / 8.9 / 7.7, 128 x 4096 x 4096 13.8 / 12.0* / 16.6, 2048 x 2048 x 2048
+    // 37.5 / 23.2 / 16.4*, 4096 x 512 x 512 8.2 / 6.8* / 6.9, 512 x 1024 x 1024 7.6* / 8.7 / 7.6.
     if(g.m > INT_MAX - 1024 || g.n > INT_MAX - 1024 || g.k > INT_MAX - 1024) return p;
     double best = 0.0;
     for(int option = 0; option < 3; option++){
@@ -722,7 +724,7 @@ static TcPlan plan_product(const Product& g, int epilogue){
             const int blocks = (k_blocks - 1) / shares + 1;
             const long long whole = tiles * shares / groups, rest = tiles * shares % groups;
             const double rounds = whole + (rest == 0 ? 0.0 : cg == 2 && whole > 0 && 2 * rest <= groups ? 0.75 : 1.0);     // a half tile loads all of A
-            const double cycles = rounds * (blocks * block + 1500.0) + (shares == 1 ? 0.0 : by_cluster ? 2500.0 : 6000.0);      // the last: a launch and a pass over the partial sums
+            const double cycles = rounds * (blocks * block + 1500.0) + (shares == 1 ? 0.0 : by_cluster ? 1500.0 + 1000.0 * shares : 6000.0);      // the last: a launch and a pass over the partial sums
             if(best == 0.0 || cycles < best){
                 best = cycles;
                 p.cg = cg; p.bn = bn; p.m_tiles = (int)m_tiles; p.n_tiles = (int)n_tiles; p.split_blocks = blocks;
