@@ -96,7 +96,7 @@ def build_tensors(force: bool = False) -> str:
     tmp = TENSORS_PATH + ".tmp"
     cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
     cmd += ["-isystem" + d for d in include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include")]]
-    cmd += [src, "-o", tmp, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    cmd += [src, "-o", tmp, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise B200RLError("g++ failed on " + src + ":\n" + res.stdout + res.stderr)

@@ -61,10 +61,6 @@ static Product weights_product(const void* x, int ldx, const void* d_pre, int ld
     g.out = const_cast<float*>(d_W); g.ld_out = input_dim;
     return g;
 }
-static bool valid_workspace(const void* workspace, size_t bytes, size_t needed){
-    return needed == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && bytes >= needed);
-}
-
 }  // namespace b200rl
 using namespace b200rl;
 
@@ -92,14 +88,12 @@ int b200rl_dense_residual_forward(int type, const void* W, int ldw, const float*
        (residual && !valid_matrix(residual, ldr, batch, output_dim, 2)) || (pre && !valid_matrix(pre, ldpre, batch, output_dim, 2)) ||
        reinterpret_cast<uintptr_t>(bias) % 4) return B200RL_ERR_INVALID_ARGUMENT;
     Product g = forward_product(W, ldw, x, ldx, batch, input_dim, output_dim);
-    const bool few = product_rows_takes(g);
-    if(!few && !valid_workspace(workspace, workspace_bytes, product_tc_workspace_bytes(g, EPI_FORWARD))) return B200RL_ERR_INVALID_ARGUMENT;
     g.bias = bias; g.scale = scale;
     g.add = residual; g.ld_add = row_pitch(ldr, batch, output_dim);
     g.pre = pre; g.ld_pre = row_pitch(ldpre, batch, output_dim);
     g.out = y; g.ld_out = row_pitch(ldy, batch, output_dim);
     g.act = activation;
-    return few ? product_rows(g, type, (cudaStream_t)stream) : product_tc(g, type, EPI_FORWARD, workspace, (cudaStream_t)stream);
+    return product_rows_takes(g) ? product_rows(g, type, (cudaStream_t)stream) : product_tc(g, type, EPI_FORWARD, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 int b200rl_dense_residual_backward_activation(int type, const void* pre, int ldpre, const void* d_y, int ldd, float scale, void* d_pre, int lddp, int rows,
@@ -129,12 +123,11 @@ int b200rl_dense_residual_backward_input(int type, const void* W, int ldw, const
        (add && !valid_matrix(add, lda, batch, input_dim, 2)) ||
        (activation_in != B200RL_ACT_IDENTITY && !valid_matrix(pre_in, ldp, batch, input_dim, 2))) return B200RL_ERR_INVALID_ARGUMENT;
     Product g = input_product(W, ldw, d_pre, ldd, batch, input_dim, output_dim);
-    if(!valid_workspace(workspace, workspace_bytes, product_tc_workspace_bytes(g, EPI_INPUT))) return B200RL_ERR_INVALID_ARGUMENT;
     g.add = add; g.ld_add = row_pitch(lda, batch, input_dim);
     g.act = activation_in;
     if(activation_in != B200RL_ACT_IDENTITY) g.pre = const_cast<void*>(pre_in); g.ld_pre = row_pitch(ldp, batch, input_dim);
     g.out = d_in; g.ld_out = row_pitch(ldi, batch, input_dim);
-    return product_tc(g, type, EPI_INPUT, workspace, (cudaStream_t)stream);
+    return product_tc(g, type, EPI_INPUT, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 int b200rl_dense_residual_backward_weights(int type, const void* x, int ldx, const void* d_pre, int ldd, float* d_W, float* d_bias, int accumulate, int batch,
@@ -152,9 +145,8 @@ int b200rl_dense_residual_backward_weights(int type, const void* x, int ldx, con
     }
     if(d_W){
         Product g = weights_product(x, ldx, d_pre, ldd, d_W, batch, input_dim, output_dim);
-        if(!valid_workspace(workspace, workspace_bytes, product_tc_workspace_bytes(g, EPI_SUM))) return B200RL_ERR_INVALID_ARGUMENT;
         g.accumulate = accumulate; g.row_sums = d_bias;
-        return product_tc(g, type, EPI_SUM, workspace, (cudaStream_t)stream);
+        return product_tc(g, type, EPI_SUM, workspace, workspace_bytes, (cudaStream_t)stream);
     }
     if(d_bias){
         B200RL_DISPATCH_16_BIT_TYPE(type, B200RL_CUDA_TRY(launch_after(column_sums_kernel<T>, dim3((output_dim - 1) / 32 + 1), dim3(1024), 0, (cudaStream_t)stream,

@@ -27,7 +27,7 @@ struct Product {
 
 // bytes of workspace for this product on the tensor cores: partial sums where k is split, copies of operands (and of fp32 results) that TMA cannot address
 size_t product_tc_workspace_bytes(const Product& g, int epilogue);
-int product_tc(const Product& g, int type, int epilogue, void* workspace, cudaStream_t s);
+int product_tc(const Product& g, int type, int epilogue, void* workspace, size_t workspace_bytes, cudaStream_t s);
 // the forward product of a few rows, without a workspace
 bool product_rows_takes(const Product& g);
 int product_rows(const Product& g, int type, cudaStream_t s);

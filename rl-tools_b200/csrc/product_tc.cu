@@ -808,9 +808,10 @@ static int launch_finish(const FinishArgs& f, cudaStream_t s){
 }
 
 template <typename T>
-static int product_tc_typed(const Product& g, int type, int epilogue, void* workspace, cudaStream_t s){
+static int product_tc_typed(const Product& g, int type, int epilogue, void* workspace, size_t workspace_bytes, cudaStream_t s){
     const TcPlan p = plan_product(g, epilogue);
     if(p.cg == 0) return B200RL_ERR_UNSUPPORTED;
+    if(p.bytes && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < p.bytes)) return B200RL_ERR_INVALID_ARGUMENT;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     Operand A = g.a, B = g.b;
     int rc;
@@ -861,8 +862,8 @@ static int product_tc_typed(const Product& g, int type, int epilogue, void* work
     if(epilogue == EPI_INPUT) return launch_tile<false, true, T, EPI_INPUT>(p, maps, a, s);
     return launch_tile<false, false, T, EPI_FORWARD>(p, maps, a, s);
 }
-int product_tc(const Product& g, int type, int epilogue, void* workspace, cudaStream_t s){
-    B200RL_DISPATCH_16_BIT_TYPE(type, return (product_tc_typed<T>(g, type, epilogue, workspace, s)))
+int product_tc(const Product& g, int type, int epilogue, void* workspace, size_t workspace_bytes, cudaStream_t s){
+    B200RL_DISPATCH_16_BIT_TYPE(type, return (product_tc_typed<T>(g, type, epilogue, workspace, workspace_bytes, s)))
 }
 int product_tc_error_get(int* word){ B200RL_CUDA_TRY(cudaMemcpyFromSymbol(word, g_product_tc_error, sizeof(int))); return B200RL_OK; }
 int product_tc_error_clear(){ const int zero = 0; B200RL_CUDA_TRY(cudaMemcpyToSymbol(g_product_tc_error, &zero, sizeof(int))); return B200RL_OK; }

@@ -3,6 +3,7 @@
 // names and defaults; the kernels are reached through the addresses of the C entry points that `bind` is given.
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -87,9 +88,14 @@ struct Operands {
     }
 };
 
+// an uninitialised tensor beside `like`; straight from the CUDA allocator where that is on a GPU (the dispatcher's way there takes as long again)
+at::Tensor empty(at::IntArrayRef shape, const at::Tensor& like, at::ScalarType type){
+    if(like.is_cuda()) return at::detail::empty_cuda(shape, type, like.device(), c10::nullopt);
+    return at::empty(shape, like.options().dtype(type));
+}
 at::Tensor workspace(size_t bytes, const at::Tensor& like, void** p){
     if(bytes == 0){ *p = nullptr; return {}; }
-    at::Tensor t = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+    at::Tensor t = empty({(int64_t)bytes}, like, at::kByte);
     *p = t.data_ptr();
     return t;
 }
@@ -103,7 +109,7 @@ struct Output {
 Output output(const char* call, const char* name, PyObject* given, bool wanted, at::IntArrayRef shape, const at::Tensor& like, at::ScalarType type, bool zero = false){
     Output o;
     if(given != Py_None){ tensor(call, name, given); o.given = given; }
-    else if(wanted) o.made = zero ? at::zeros(shape, like.options().dtype(type)) : at::empty(shape, like.options().dtype(type));
+    else if(wanted) o.made = zero ? at::zeros(shape, like.options().dtype(type)) : empty(shape, like, type);
     return o;
 }
 void is_matrix(const char* call, const char* name, const at::Tensor* t){
