@@ -65,21 +65,37 @@ struct NormBackward {
     float scale, epsilon;
 };
 
-// Sums of N values over the threads of a row (one warp, or the whole CTA); every thread gets them. `buffer` is used in turns, so one barrier per call is enough.
+// Sums of N values over the threads of a row (one warp, or the whole CTA); every thread gets them. Within a warp the lanes share the values out first: each exchange halves what a
+// lane carries, so four values take six exchanges instead of twenty. `buffer` is used in turns, so one barrier per call is enough.
 template <int TPR, int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], float (*buffer)[4][TPR / 32], int& turn){
-    static_assert(N <= 4);
+    static_assert(N == 1 || N == 2 || N == 4);
+    const int lane = threadIdx.x & 31;
+    float mine = v[0];                                       // of value lane / (32 / N)
+    if constexpr(N == 4){
+        const bool upper = lane & 16, odd = lane & 8;
+        float a = upper ? v[2] : v[0], b = upper ? v[3] : v[1];
+        a += __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[2], 16);
+        b += __shfl_xor_sync(0xffffffffu, upper ? v[1] : v[3], 16);
+        mine = odd ? b : a;
+        mine += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+    }
+    if constexpr(N == 2){
+        const bool upper = lane & 16;
+        mine = upper ? v[1] : v[0];
+        mine += __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[1], 16);
+    }
 #pragma unroll
-    for(int o = 16; o > 0; o >>= 1)
+    for(int o = 16 / N; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if constexpr(TPR == 32){
 #pragma unroll
-        for(int i = 0; i < N; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    if constexpr(TPR > 32){
+        for(int i = 0; i < N; i++) v[i] = __shfl_sync(0xffffffffu, mine, i * (32 / N));
+    }
+    else{
         float (&shared)[4][TPR / 32] = buffer[turn];
         turn ^= 1;
         const int warp = threadIdx.x >> 5;
-        if((threadIdx.x & 31) == 0)
-#pragma unroll
-            for(int i = 0; i < N; i++) shared[i][warp] = v[i];
+        if((lane & (32 / N - 1)) == 0) shared[lane / (32 / N)][warp] = mine;
         __syncthreads();
 #pragma unroll
         for(int i = 0; i < N; i++){
@@ -201,7 +217,7 @@ __device__ __forceinline__ void normalise(const R& row, int kind, float2 (&v)[P]
     for(int i = 0; i < P; i++) squares = fma2(v[i], v[i], squares);
     float s[1] = {across(squares)};
     row_sums<TPR>(s, buffer, turn);
-    const float rstd = 1.0f / sqrtf(s[0] * inv + epsilon);
+    const float rstd = rsqrtf(s[0] * inv + epsilon);
 #pragma unroll
     for(int i = 0; i < P; i++) v[i] = mul2(v[i], both(rstd));
 }
@@ -397,7 +413,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, backward_ctas<T>(TPR, E
             float s[4] = {across(xx), across(uu), across(gg), across(gx)};
             row_sums<TPR>(s, buffer, turn);
             if(pre){
-                const float rstd = 1.0f / sqrtf(s[0] * inv + a.epsilon), mean = a.pre == B200RL_NORM_LAYER ? s[2] * inv : 0.0f, along = s[3] * rstd * inv;
+                const float rstd = rsqrtf(s[0] * inv + a.epsilon), mean = a.pre == B200RL_NORM_LAYER ? s[2] * inv : 0.0f, along = s[3] * rstd * inv;
 #pragma unroll
                 for(int i = 0; i < E / 4; i++){
                     const float4 w = kept.at(K::PRE_WEIGHT, i);
@@ -409,7 +425,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, backward_ctas<T>(TPR, E
                 }
                 if(a.pre == B200RL_NORM_LAYER) row.clear_outside(d);     // the post norm sums what lies behind the row's end too
             }
-            if(post) rstd_u = 1.0f / sqrtf(s[1] * inv + a.epsilon);
+            if(post) rstd_u = rsqrtf(s[1] * inv + a.epsilon);
         }
         if(a.d_residual) row.store(a.d_residual, r * a.lddr, d);
         if(!a.branch) continue;
