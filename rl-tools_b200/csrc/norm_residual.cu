@@ -522,19 +522,32 @@ __device__ __forceinline__ GatePieces gate_pieces(const NormBackward& a, long lo
     return {group, w, (int)((end - 1) / a.rows_per_worker) - w + 1};
 }
 
-// The sums over the workers, in their order: blockIdx.y < n_sums the parameter gradients, behind them gate rows (few, of many pieces). 32 columns a CTA, 16 threads a column.
+// The sums over the workers, in their order, one launch for all. The first CTAs take the parameter gradients that are asked for and, if gate rows that several workers share are few
+// (and have many pieces), those: 32 columns a CTA, 16 threads a column. Behind them, for many gate rows of few pieces, a CTA takes 512 columns of the gate row that lies across
+// the boundary between one worker and the next, a thread a column.
 template <typename T>
-__global__ void __launch_bounds__(512) norm_backward_sums_kernel(NormBackward a){
+__global__ void __launch_bounds__(512) norm_backward_sums_kernel(NormBackward a, int few_gates){
     __shared__ float shared[16][33];
     after_predecessor();
-    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    const bool parameter = (int)blockIdx.y < a.n_sums;
-    const int index = parameter ? a.sums[blockIdx.y] : 0;
+    const int columns = (a.dim - 1) / 32 + 1, sum_ctas = (a.n_sums + few_gates) * columns;
+    if((int)blockIdx.x >= sum_ctas){
+        const int parts = (a.dim - 1) / 512 + 1, at = blockIdx.x - sum_ctas, worker = at / parts, c = (at - worker * parts) * 512 + threadIdx.x;
+        const long long row = (worker + 1ll) * a.rows_per_worker;                       // the next worker's first row
+        const GatePieces g = gate_pieces(a, row / a.gate_rows);
+        if(c >= a.dim || g.first != worker) return;                                     // a gate row begins at the boundary, or its first boundary is an earlier one
+        float v = a.pieces[(2ll * g.first + 1) * a.dim + c];
+        for(int i = 1; i < g.n; i++) v += a.pieces[2ll * (g.first + i) * a.dim + c];
+        static_cast<T*>(a.d_gate)[g.group * a.lddg + c] = from_float<T>(v);
+        return;
+    }
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, what = blockIdx.x / columns, c = (blockIdx.x - what * columns) * 32 + lane;
+    const bool parameter = what < a.n_sums;
+    const int index = parameter ? a.sums[what] : 0;
     const float* part; long long stride; int n, skip = 0;
     GatePieces g{};
     if(parameter){ part = a.partials + (long long)index * a.workers * a.dim; stride = a.dim; n = a.workers; }
     else{
-        g = gate_pieces(a, blockIdx.y - a.n_sums);
+        g = gate_pieces(a, what - a.n_sums);
         if(g.n == 1) return;
         part = a.pieces + 2ll * g.first * a.dim; stride = 2ll * a.dim; n = g.n; skip = a.dim;
     }
@@ -554,18 +567,6 @@ __global__ void __launch_bounds__(512) norm_backward_sums_kernel(NormBackward a)
     for(int i = 1; i < 16; i++) v += shared[i][lane];
     if(parameter){ float* out = a.d_params[index] + c; *out = a.accumulate ? *out + v : v; }
     else static_cast<T*>(a.d_gate)[g.group * a.lddg + c] = from_float<T>(v);
-}
-// The same for many gate rows of few pieces: blockIdx.y is the worker behind a boundary, a thread a column.
-template <typename T>
-__global__ void __launch_bounds__(256) norm_backward_gates_kernel(NormBackward a){
-    after_predecessor();
-    const long long row = (blockIdx.y + 1ll) * a.rows_per_worker;                   // the worker's first row
-    const GatePieces g = gate_pieces(a, row / a.gate_rows);
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if(c >= a.dim || g.first != (int)blockIdx.y) return;                            // a gate row begins at the boundary, or its first boundary is an earlier one
-    float v = a.pieces[(2ll * g.first + 1) * a.dim + c];
-    for(int i = 1; i < g.n; i++) v += a.pieces[2ll * (g.first + i) * a.dim + c];
-    static_cast<T*>(a.d_gate)[g.group * a.lddg + c] = from_float<T>(v);
 }
 
 // Workers of the backward pass, and the consecutive rows that each takes: as many as are resident at once, a row each where there are fewer rows than that.
@@ -698,15 +699,10 @@ int b200rl_norm_residual_backward(int type, int post, const float* post_weight, 
         return gate ? launch_backward<T, V, TPR, E, false, true>(a, st) : launch_backward<T, V, TPR, E, false, false>(a, st);
     }))
     if(rc) return rc;
-    const bool shared_gates = d_gate && a.workers > 1 && gate_rows > 1, few_gates = shared_gates && gates <= 32;
-    if(few_gates || a.n_sums){
-        const dim3 grid((dim + 31) / 32, a.n_sums + (few_gates ? gates : 0));
-        B200RL_DISPATCH_TYPE(type, B200RL_CUDA_TRY(launch_after(norm_backward_sums_kernel<T>, grid, dim3(512), 0, (cudaStream_t)stream, a)))
-    }
-    if(shared_gates && !few_gates){
-        const dim3 grid((dim + 255) / 256, a.workers - 1);
-        B200RL_DISPATCH_TYPE(type, B200RL_CUDA_TRY(launch_after(norm_backward_gates_kernel<T>, grid, dim3(256), 0, (cudaStream_t)stream, a)))
-    }
+    const bool shared_gates = d_gate && a.workers > 1 && gate_rows > 1;
+    const int few_gates = shared_gates && gates <= 32 ? gates : 0;
+    const int ctas = (a.n_sums + few_gates) * ((dim - 1) / 32 + 1) + (shared_gates && !few_gates ? (a.workers - 1) * ((dim - 1) / 512 + 1) : 0);
+    if(ctas) B200RL_DISPATCH_TYPE(type, B200RL_CUDA_TRY(launch_after(norm_backward_sums_kernel<T>, dim3(ctas), dim3(512), 0, (cudaStream_t)stream, a, few_gates)))
     return B200RL_OK;
 }
 

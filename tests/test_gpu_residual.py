@@ -325,7 +325,7 @@ def test_the_first_call_of_a_process_may_be_captured(lib):
 
 
 # ---- norms -------------------------------------------------------------------------------------------------------------------------------------
-NORM_SIZES = [(1, 1), (1, 4096), (3, 5), (7, 64), (50, 257), (33, 512), (130, 777), (64, 1024), (20, 2048), (9, 2049), (300, 100), (5, 4097), (4, 8192), (700, 33), (2500, 16)]
+NORM_SIZES = [(1, 1), (1, 4096), (3, 5), (7, 64), (50, 257), (33, 512), (130, 777), (64, 1024), (20, 2048), (9, 2049), (300, 100), (5, 4097), (4, 8192), (700, 33), (2500, 16), (5003, 40), (2000, 600)]
 
 
 def norm_inputs(R, D, dtype, post, pre, gate_rows, bias, layout, seed):
