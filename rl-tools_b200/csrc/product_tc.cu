@@ -252,40 +252,60 @@ template <typename T, int EPI> __device__ __forceinline__ void finish_whole_or_p
     if(row0 + 32 <= a.m && col + 32 <= a.n){ B200RL_DISPATCH_RESIDUAL_ACT(a.act, (finish_slab<T, EPI, ACT, true>(a, slab, o, bias, row0, col, lane))) }
     else { B200RL_DISPATCH_RESIDUAL_ACT(a.act, (finish_slab<T, EPI, ACT, false>(a, slab, o, bias, row0, col, lane))) }
 }
-// The same where rows start at odd addresses: a lane has a column
+// The same where rows start at odd addresses: a lane has a column. Eight rows at a time, so that their operands are under way together and the places in the slab differ in
+// constants; WHOLE: all of the slab's rows are there.
+template <typename T, int EPI, int ACT, bool WHOLE>
+__device__ __forceinline__ void finish_rows(const TcArgs& a, const uint8_t* slab, int row0, int col, int lane){
+    const float bias = EPI == EPI_FORWARD && a.bias ? a.bias[col] : 0.0f;
+    const int rows = WHOLE ? 32 : min(32, a.m - row0);
+    const T* add_at = a.add ? static_cast<const T*>(a.add) + (long long)row0 * a.ld_add + col : nullptr;
+    T* pre_at = a.pre ? static_cast<T*>(a.pre) + (long long)row0 * a.ld_pre + col : nullptr;
+    T* out_at = static_cast<T*>(a.out) + (long long)row0 * a.ld_out + col;
+    const uint32_t from = tc::smem_u32(slab) + ((lane >> 2) << 4) + (lane & 3) * 4;
+    const long long ld_add = a.ld_add, ld_pre = a.ld_pre, ld_out = a.ld_out;
+#pragma unroll 1
+    for(int r0 = 0; r0 < rows; r0 += 8){
+        T add_raw[8], pre_raw[8];
+        if(add_at)
+#pragma unroll
+            for(int r = 0; r < 8; r++, add_at += ld_add) if(WHOLE || r0 + r < rows) add_raw[r] = *add_at;
+        if constexpr(EPI == EPI_INPUT && ACT != B200RL_ACT_IDENTITY)
+#pragma unroll
+            for(int r = 0; r < 8; r++, pre_at += ld_pre) if(WHOLE || r0 + r < rows) pre_raw[r] = *pre_at;
+        float x[8];
+#pragma unroll
+        for(int r = 0; r < 8; r++) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x[r]) : "r"((from ^ (r << 4)) + (r0 + r) * 128) : "memory");
+        float2 v[4] = {make_float2(x[0], x[1]), make_float2(x[2], x[3]), make_float2(x[4], x[5]), make_float2(x[6], x[7])};
+        if constexpr(EPI == EPI_FORWARD){
+            if(a.bias)
+#pragma unroll
+                for(int r = 0; r < 4; r++) v[r] = add2(v[r], both(bias));
+            if(pre_at)
+#pragma unroll
+                for(int r = 0; r < 8; r++, pre_at += ld_pre) if(WHOLE || r0 + r < rows) *pre_at = from_float<T>(r & 1 ? v[r / 2].y : v[r / 2].x);
+            activate_pairs<ACT>(v);
+#pragma unroll
+            for(int r = 0; r < 4; r++) v[r] = mul2(v[r], both(a.scale));
+        }
+        if(add_at)
+#pragma unroll
+            for(int r = 0; r < 4; r++) v[r] = add2(v[r], make_float2(to_float(add_raw[2 * r]), to_float(add_raw[2 * r + 1])));
+        if constexpr(EPI == EPI_INPUT && ACT != B200RL_ACT_IDENTITY){
+            float p[8];
+#pragma unroll
+            for(int r = 0; r < 8; r++) p[r] = to_float(pre_raw[r]);
+            times_slope_pairs<ACT>(v, p);
+        }
+#pragma unroll
+        for(int r = 0; r < 8; r++, out_at += ld_out) if(WHOLE || r0 + r < rows) *out_at = from_float<T>(r & 1 ? v[r / 2].y : v[r / 2].x);
+    }
+}
 template <typename T, int EPI>
 __device__ __forceinline__ void finish_slab_by_rows(const TcArgs& a, const uint8_t* slab, int row0, int col0, int lane){
     const int col = col0 + lane;
     if(col >= a.n) return;
-    const float bias = EPI == EPI_FORWARD && a.bias ? a.bias[col] : 0.0f;
-    const int rows = min(32, a.m - row0);
-#pragma unroll 1
-    for(int r0 = 0; r0 < rows; r0 += 8){
-        float add[8], x[8];                                              // eight rows' operands under way together
-#pragma unroll
-        for(int r = 0; r < 8; r++) add[r] = a.add && r0 + r < rows ? to_float(static_cast<const T*>(a.add)[(long long)(row0 + r0 + r) * a.ld_add + col]) : 0.0f;
-#pragma unroll
-        for(int r = 0; r < 8; r++) x[r] = slab_element(slab, r0 + r, lane) + bias;
-        if constexpr(EPI == EPI_FORWARD){
-            if(a.pre)
-#pragma unroll
-                for(int r = 0; r < 8; r++) if(r0 + r < rows) static_cast<T*>(a.pre)[(long long)(row0 + r0 + r) * a.ld_pre + col] = from_float<T>(x[r]);
-            B200RL_DISPATCH_RESIDUAL_ACT(a.act, activate8<ACT>(x))
-#pragma unroll
-            for(int r = 0; r < 8; r++) x[r] = fmaf(a.scale, x[r], add[r]);
-        }
-        else{
-#pragma unroll
-            for(int r = 0; r < 8; r++) x[r] += add[r];
-            if(a.act != B200RL_ACT_IDENTITY){
-#pragma unroll
-                for(int r = 0; r < 8; r++) add[r] = r0 + r < rows ? to_float(static_cast<const T*>(a.pre)[(long long)(row0 + r0 + r) * a.ld_pre + col]) : 0.0f;
-                B200RL_DISPATCH_RESIDUAL_ACT(a.act, times_slope8<ACT>(x, add))
-            }
-        }
-#pragma unroll
-        for(int r = 0; r < 8; r++) if(r0 + r < rows) static_cast<T*>(a.out)[(long long)(row0 + r0 + r) * a.ld_out + col] = from_float<T>(x[r]);
-    }
+    if(row0 + 32 <= a.m){ B200RL_DISPATCH_RESIDUAL_ACT(a.act, (finish_rows<T, EPI, ACT, true>(a, slab, row0, col, lane))) }
+    else { B200RL_DISPATCH_RESIDUAL_ACT(a.act, (finish_rows<T, EPI, ACT, false>(a, slab, row0, col, lane))) }
 }
 // A slab of an fp32 result
 __device__ __forceinline__ void store_sums(const TcArgs& a, const uint8_t* slab, int z, int row0, int col0, int lane){
@@ -315,7 +335,8 @@ __device__ __forceinline__ void store_sums(const TcArgs& a, const uint8_t* slab,
 template <typename T>
 __device__ __forceinline__ void sum_rows(const TcArgs& a, float* shared, int tid, int warp, int lane);
 
-template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI>
+// FAST: 16-bit outputs, add and pre by 16-byte accesses (both epilogues in one kernel take registers from one another: 4096 x 1024 x 4096 with everything 47 us instead of 41)
+template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI, bool FAST>
 __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                 const __grid_constant__ TcArgs a){
     constexpr int STAGES = stage_count(CG, BN);
@@ -480,7 +501,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 const uint32_t b = acc & 1, phase = (acc >> 1) & 1;
                 acc++;
                 SlabOperands o;
-                if(a.fast && sharers == 1) fetch_slab<T, EPI>(o, a, row0, col0, lane);
+                if(FAST && sharers == 1) fetch_slab<T, EPI>(o, a, row0, col0, lane);
                 if(!warp_wait(acc_full + b, phase)){ ok = false; break; }
                 tc::fence_after_thread_sync();
                 uint32_t r[32];
@@ -500,14 +521,20 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     tc::tmem_wait_ld();
                     __syncwarp();                                        // the slab before has been read
                     slab_in(slab, r, lane);
-                    if(j + 1 < slabs) tc::tmem_ld_32x32(tmem + lanes + b * BN + tile_col + (j + 1) * 32, r);
+                    if(j + 1 < slabs){ if(FAST) tc::tmem_ld_32x32(tmem + lanes + b * BN + tile_col + (j + 1) * 32, r); }
                     else tc::fence_before_thread_sync();
                     __syncwarp();
                     if(j + 1 == slabs && lane == 0) arrive_at_leader<CG>(acc_empty + b);
-                    if(row0 >= a.m || col >= a.n) continue;
-                    if(!a.fast){ finish_slab_by_rows<T, EPI>(a, slab, row0, col, lane); continue; }
-                    finish_whole_or_part<T, EPI>(a, slab, o, row0, col, lane);
-                    if(j + 1 < slabs) fetch_slab<T, EPI>(o, a, row0, col + 32, lane);
+                    if constexpr(!FAST){
+                        if(row0 < a.m && col < a.n) finish_slab_by_rows<T, EPI>(a, slab, row0, col, lane);
+                        __syncwarp();
+                        if(j + 1 < slabs) tc::tmem_ld_32x32(tmem + lanes + b * BN + tile_col + (j + 1) * 32, r);      // not ahead: the registers are in use
+                    }
+                    else{
+                        if(row0 >= a.m || col >= a.n) continue;
+                        finish_whole_or_part<T, EPI>(a, slab, o, row0, col, lane);
+                        if(j + 1 < slabs) fetch_slab<T, EPI>(o, a, row0, col + 32, lane);
+                    }
                 }
             }
         }
@@ -525,7 +552,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     const int col = i.n * BN + group * CW + j * 32;
                     if((w * SLABS + j) % sharers != share || col >= a.n) continue;
                     SlabOperands o;
-                    if(a.fast) fetch_slab<T, EPI>(o, a, row0, col, lane);
+                    if constexpr(FAST) fetch_slab<T, EPI>(o, a, row0, col, lane);
                     uint8_t* slab = staging + w * STAGING;
                     __syncwarp();
 #pragma unroll 1
@@ -544,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                         for(int c = 0; c < 4; c++) *reinterpret_cast<float4*>(slab + half * 2048 + (c * 32 + lane) * 16) = sum[c];
                     }
                     __syncwarp();
-                    if(a.fast) finish_whole_or_part<T, EPI>(a, slab, o, row0, col, lane);
+                    if constexpr(FAST) finish_whole_or_part<T, EPI>(a, slab, o, row0, col, lane);
                     else finish_slab_by_rows<T, EPI>(a, slab, row0, col, lane);
                 }
             __syncwarp();
@@ -647,6 +674,34 @@ __global__ void __launch_bounds__(256) finish_kernel(FinishArgs f){
         }
 }
 
+// `count` elements (1 to 8) at any address, 0 behind them: the one or two 16-byte pieces of memory that they lie in (no piece without one of them is touched), shifted into place
+__device__ __forceinline__ uint4 unaligned_eight(const uint16_t* p, int count){
+    const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15);
+    const uint4* piece = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - shift);
+    const uint4 lo = piece[0];
+    uint4 hi = make_uint4(0, 0, 0, 0);
+    if(shift + 2 * count > 16) hi = piece[1];
+    uint32_t w[7] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z};
+    uint32_t last = hi.w;
+    if(shift & 8){
+#pragma unroll
+        for(int i = 0; i < 5; i++) w[i] = w[i + 2];
+        w[5] = last; w[6] = 0; last = 0;
+    }
+    if(shift & 4){
+#pragma unroll
+        for(int i = 0; i < 6; i++) w[i] = w[i + 1];
+        w[6] = last;
+    }
+    uint32_t out[4];
+#pragma unroll
+    for(int i = 0; i < 4; i++){
+        const uint32_t v = shift & 2 ? w[i] >> 16 | w[i + 1] << 16 : w[i];
+        out[i] = 2 * i + 1 < count ? v : 2 * i < count ? v & 0xFFFFu : 0u;
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
 // Rows of 16-bit elements at any address -> rows that start on 16-byte boundaries, eight elements a thread; one operand or both
 struct AlignRows { const uint16_t* src; long long ld; uint16_t* dst; long long ld_dst, rows; int cols; };
 __global__ void __launch_bounds__(256) align_rows_kernel(AlignRows first, AlignRows second){
@@ -658,10 +713,7 @@ __global__ void __launch_bounds__(256) align_rows_kernel(AlignRows first, AlignR
         const long long at = one ? i : i - chunks_1;
         const int chunks = (int)(o.ld_dst / 8);
         const long long r = at / chunks; const int c = (int)(at - r * chunks) * 8;
-        union { uint4 v; uint16_t e[8]; } u;
-#pragma unroll
-        for(int j = 0; j < 8; j++) u.e[j] = c + j < o.cols ? o.src[r * o.ld + c + j] : (uint16_t)0;
-        *reinterpret_cast<uint4*>(o.dst + r * o.ld_dst + c) = u.v;
+        *reinterpret_cast<uint4*>(o.dst + r * o.ld_dst + c) = unaligned_eight(o.src + r * o.ld + c, min(8, o.cols - c));
     }
 }
 
@@ -764,9 +816,9 @@ static TcPlan plan_product(const Product& g, int epilogue){
 }
 size_t product_tc_workspace_bytes(const Product& g, int epilogue){ return plan_product(g, epilogue).bytes; }
 
-template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI>
+template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI, bool FAST>
 static int launch_tc(const CUtensorMap (&maps)[2], const TcArgs& a, cudaStream_t s){
-    auto* kernel = product_tc_kernel<CG, BN, A_ROWS, B_ROWS, T, EPI>;
+    auto* kernel = product_tc_kernel<CG, BN, A_ROWS, B_ROWS, T, EPI, FAST>;
     static std::atomic<int> groups[MAX_DEVICES];           // tiles that run at the same time: 0 until the kernel is set up on the device
     int dev = 0, sms = 0;
     int rc = current_device(&dev);
@@ -795,11 +847,11 @@ static int launch_tc(const CUtensorMap (&maps)[2], const TcArgs& a, cudaStream_t
     B200RL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], a));
     return B200RL_OK;
 }
-template <bool A_ROWS, bool B_ROWS, typename T, int EPI>
+template <bool A_ROWS, bool B_ROWS, typename T, int EPI, bool FAST>
 static int launch_tile(const TcPlan& p, const CUtensorMap (&maps)[2], const TcArgs& a, cudaStream_t s){
-    if(p.cg == 2) return launch_tc<2, 256, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
-    if(p.bn == 128) return launch_tc<1, 128, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
-    return launch_tc<1, 64, A_ROWS, B_ROWS, T, EPI>(maps, a, s);
+    if(p.cg == 2) return launch_tc<2, 256, A_ROWS, B_ROWS, T, EPI, FAST>(maps, a, s);
+    if(p.bn == 128) return launch_tc<1, 128, A_ROWS, B_ROWS, T, EPI, FAST>(maps, a, s);
+    return launch_tc<1, 64, A_ROWS, B_ROWS, T, EPI, FAST>(maps, a, s);
 }
 static int launch_finish(const FinishArgs& f, cudaStream_t s){
     const long long blocks = ((long long)f.a.m * f.a.n + 255) / 256;
@@ -855,12 +907,12 @@ static int product_tc_typed(const Product& g, int type, int epilogue, void* work
             f.row_sums = p.splits > 1 ? b.sums : nullptr;
             f.a.sums_accumulate = g.accumulate;
         }
-        if((rc = launch_tile<true, true, T, EPI_SUM>(p, maps, b, s)) || !p.partial) return rc;
+        if((rc = launch_tile<true, true, T, EPI_SUM, true>(p, maps, b, s)) || !p.partial) return rc;
         return launch_finish(f, s);
     }
     a.fast = rows_aligned(g.out, g.ld_out, 2) && (!g.add || rows_aligned(g.add, g.ld_add, 2)) && (!g.pre || rows_aligned(g.pre, g.ld_pre, 2));
-    if(epilogue == EPI_INPUT) return launch_tile<false, true, T, EPI_INPUT>(p, maps, a, s);
-    return launch_tile<false, false, T, EPI_FORWARD>(p, maps, a, s);
+    if(epilogue == EPI_INPUT) return a.fast ? launch_tile<false, true, T, EPI_INPUT, true>(p, maps, a, s) : launch_tile<false, true, T, EPI_INPUT, false>(p, maps, a, s);
+    return a.fast ? launch_tile<false, false, T, EPI_FORWARD, true>(p, maps, a, s) : launch_tile<false, false, T, EPI_FORWARD, false>(p, maps, a, s);
 }
 int product_tc(const Product& g, int type, int epilogue, void* workspace, size_t workspace_bytes, cudaStream_t s){
     B200RL_DISPATCH_16_BIT_TYPE(type, return (product_tc_typed<T>(g, type, epilogue, workspace, workspace_bytes, s)))
