@@ -11,7 +11,7 @@
 // Products of few tiles share each tile's k among the CTAs of a cluster, which add up through one another's shared memory.
 //
 // Bound by the tensor cores where the products are long: 16384 x 4096 x 4096 bfloat16 336 us = 1,637 TFLOP/s (the tensor pipe busy 84 to 92% of the cycles; the same product
-// in the library's form takes 340 to 348), 4096 x 1024 x 4096 27 us, with gelu and pre-activations kept 34. A stage's operands take 64 bytes a cycle and multiprocessor from L2, all
+// in the library's form takes 340 to 348), 4096 x 1024 x 4096 26 us, with gelu and pre-activations kept 34. A stage's operands take 64 bytes a cycle and multiprocessor from L2, all
 // that it gives; tiles of 256 x 256 over a pair are what the tensor memory holds twice (128 x 128 by one CTA: 740 us). Small products are bound by the way through the kernel
 // (256 x 256 x 256 4.5 us: 0.9 until the first operands are there, 1 for the products, 0.8 for the epilogue, the rest launch).
 #include "product.cuh"
@@ -335,7 +335,7 @@ __device__ __forceinline__ void store_sums(const TcArgs& a, const uint8_t* slab,
 template <typename T>
 __device__ __forceinline__ void sum_rows(const TcArgs& a, float* shared, int tid, int warp, int lane);
 
-// FAST: 16-bit outputs, add and pre by 16-byte accesses (both epilogues in one kernel take registers from one another: 4096 x 1024 x 4096 with everything 47 us instead of 41)
+// FAST: 16-bit outputs, add and pre by 16-byte accesses (both epilogues in one kernel take registers from one another: 4096 x 1024 x 4096 with everything 41 us instead of 39)
 template <int CG, int BN, bool A_ROWS, bool B_ROWS, typename T, int EPI, bool FAST>
 __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                 const __grid_constant__ TcArgs a){
