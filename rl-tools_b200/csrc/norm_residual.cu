@@ -178,18 +178,19 @@ struct Row {
             if(column(i) < dim) store_elements(row + column(i), e);
         }
     }
+    // ordinary loads: read-only ones could be moved in front of the wait for the kernel before, which may be the optimizer step that writes these parameters
     __device__ __forceinline__ void parameters(const float* p, float fill, float (&v)[E]) const {
         if(VEC > 1 && reinterpret_cast<uintptr_t>(p) % 16 == 0){
 #pragma unroll
             for(int e = 0; e < E; e += 4){
                 float4 q = make_float4(fill, fill, fill, fill);
-                if(p && inside(e)) q = __ldg(reinterpret_cast<const float4*>(p + column(e / VEC) + e % VEC));
+                if(p && inside(e)) q = *reinterpret_cast<const float4*>(p + column(e / VEC) + e % VEC);
                 v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
             }
         }
         else
 #pragma unroll
-            for(int e = 0; e < E; e++) v[e] = p && inside(e) ? __ldg(p + column(e / VEC) + e % VEC) : fill;
+            for(int e = 0; e < E; e++) v[e] = p && inside(e) ? p[column(e / VEC) + e % VEC] : fill;
     }
 };
 
