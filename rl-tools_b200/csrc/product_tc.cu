@@ -475,8 +475,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     for(int j = 0; j < SLABS; j++){
                         if(j >= slabs) break;
                         uint32_t r[32];
-                        tc::tmem_ld_32x32(tmem + lanes + b * BN + tile_col + j * 32, r);
-                        tc::tmem_wait_ld();
+                        tc::tmem_load_32x32(tmem + lanes + b * BN + tile_col + j * 32, r);
 #pragma unroll
                         for(int c = 0; c < 32; c++) sum[j][c] += __uint_as_float(r[c]);
                     }
@@ -508,28 +507,21 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 if(sharers > 1){                                         // one tile a cluster: its sums go where the operands were
 #pragma unroll
                     for(int j = 0; j < SLABS; j++){
-                        tc::tmem_ld_32x32(tmem + lanes + b * BN + group * CW + j * 32, r);
-                        tc::tmem_wait_ld();
+                        tc::tmem_load_32x32(tmem + lanes + b * BN + group * CW + j * 32, r);
                         slab_in(base + (w * SLABS + j) * 4096, r, lane);
                     }
                     break;
                 }
-                tc::tmem_ld_32x32(tmem + lanes + b * BN + tile_col, r);
 #pragma unroll 1
                 for(int j = 0; j < slabs; j++){
                     const int col = col0 + j * 32;
-                    tc::tmem_wait_ld();
+                    tc::tmem_load_32x32(tmem + lanes + b * BN + tile_col + j * 32, r);
                     __syncwarp();                                        // the slab before has been read
                     slab_in(slab, r, lane);
-                    if(j + 1 < slabs){ if(FAST) tc::tmem_ld_32x32(tmem + lanes + b * BN + tile_col + (j + 1) * 32, r); }
-                    else tc::fence_before_thread_sync();
+                    if(j + 1 == slabs) tc::fence_before_thread_sync();
                     __syncwarp();
                     if(j + 1 == slabs && lane == 0) arrive_at_leader<CG>(acc_empty + b);
-                    if constexpr(!FAST){
-                        if(row0 < a.m && col < a.n) finish_slab_by_rows<T, EPI>(a, slab, row0, col, lane);
-                        __syncwarp();
-                        if(j + 1 < slabs) tc::tmem_ld_32x32(tmem + lanes + b * BN + tile_col + (j + 1) * 32, r);      // not ahead: the registers are in use
-                    }
+                    if constexpr(!FAST){ if(row0 < a.m && col < a.n) finish_slab_by_rows<T, EPI>(a, slab, row0, col, lane); }
                     else{
                         if(row0 >= a.m || col >= a.n) continue;
                         finish_whole_or_part<T, EPI>(a, slab, o, row0, col, lane);

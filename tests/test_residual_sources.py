@@ -21,3 +21,8 @@ def test_no_load_may_pass_the_wait_for_the_kernel_before(name):
     """These kernels start while the kernel before them may still write what they read (an optimizer step and the norm behind it). Their wait holds ordinary loads; a read-only load
     may be moved in front of it."""
     assert not re.findall(r"__ldg\b|__restrict__|ld\.global\.nc|ldu\b", code(name))
+
+
+def test_no_register_of_a_tensor_memory_load_is_named_before_its_wait():
+    """What tcgen05.ld writes is there behind tcgen05.wait::ld alone. With both in one statement no copy, spill or loop variable of the registers can lie between them."""
+    assert not re.findall(r"tmem_ld_32x32|tmem_wait_ld|tcgen05\.ld", code("product_tc.cu"))
