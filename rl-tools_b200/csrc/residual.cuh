@@ -68,35 +68,45 @@ __device__ __forceinline__ float2 both(float v){ return make_float2(v, v); }
 __device__ __forceinline__ float across(float2 v){ return v.x + v.y; }
 
 // Activations and their slopes: the framework's definitions and two more, with few instructions, since they run on every element that a product leaves (a tile of 128 x 256 over
-// 1024 k takes the tensor core 8,200 cycles; with erff the activation alone took 9,000 of the multiprocessor's, this way about 3,000). Errors stay below 1e-6, a thousandth of the
-// rounding to 16 bits.
-//   Phi(x): erfc by Abramowitz and Stegun, "Handbook of Mathematical Functions", 7.1.26: erfc(z) = t (a1 + t (a2 + ...)) exp(-z^2) within 1.5e-7, t = 1 / (1 + p z), z >= 0
-// Phi(x) = 1/2 + sign(x) (1/2 - erfc(|x| / sqrt 2) / 2). Two at a time; the two reciprocals are one, of the product (|x| is cut at 20, where the density has long been 0).
-struct NormalPair { float2 phi, density; };                              // Phi(x) and exp(-x^2 / 2)
+// 1024 k takes the tensor core 8,200 cycles; with erff the activation alone took 9,000 of the multiprocessor's, this way about 3,000).
+// The normal distribution: Phi(-|x|) = exp(-x^2 / 2) P(t), t = 1 / (1 + c z), z = |x| / sqrt 2, with P(t) = t (b1 + t (b2 + ... t b6)) in place of exp(z^2) erfc(z) / 2. P and c are the
+// minimax fit of this form over 0 <= z <= 9.4, by linear programming on the relative error weighted by max(erfc(z), 1/30): off by 4e-7 of the value at 0, by at most 1.2e-5 of it
+// in the tail, where the values themselves vanish, a three-hundredth of half a step of bfloat16 and a fortieth of float16's, whatever x is. (Nothing is subtracted from 1 for
+// x < 0: it would leave nothing of the tail.) Two at a time; the two reciprocals are one, of the product (|x| is cut at 20, where the density has long been 0).
+struct NormalPair { float2 size, tail, density; };                       // |x| up to 20, -Phi(-|x|), exp(-x^2 / 2)
 __device__ __forceinline__ NormalPair normal_pair(float2 x){
-    const float2 d = fma2(make_float2(fminf(fabsf(x.x), 20.0f), fminf(fabsf(x.y), 20.0f)), both(0.3275911f * 0.70710678118654752f), both(1.0f));
+    NormalPair n;
+    n.size = make_float2(fminf(fabsf(x.x), 20.0f), fminf(fabsf(x.y), 20.0f));
+    const float2 d = fma2(n.size, both(0.42263395f * 0.70710678118654752f), both(1.0f));
     const float r = __fdividef(1.0f, d.x * d.y);
     const float2 t = mul2(make_float2(d.y, d.x), both(r));
     const float2 e = mul2(mul2(x, x), both(-0.5f));
-    NormalPair n;
     n.density = make_float2(__expf(e.x), __expf(e.y));
-    float2 p = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
-    p = fma2(t, p, both(0.5f * 1.421413741f));
-    p = fma2(t, p, both(0.5f * -0.284496736f));
-    p = mul2(mul2(t, fma2(t, p, both(0.5f * 0.254829592f))), n.density);
-    const float2 off = fma2(p, both(-1.0f), both(0.5f));                  // >= 0 but for its last bits
-    n.phi = add2(make_float2(copysignf(off.x, x.x), copysignf(off.y, x.y)), both(0.5f));
+    float2 p = fma2(t, both(0.0805534029f), both(-0.229271916f));
+    p = fma2(t, p, both(0.0306924702f));
+    p = fma2(t, p, both(-0.15041971f));
+    p = fma2(t, p, both(-0.111817672f));
+    n.tail = mul2(mul2(t, fma2(t, p, both(-0.119736333f))), n.density);
     return n;
+}
+__device__ __forceinline__ float2 gelu_pair(float2 x){                   // x Phi(x) = max(x, 0) - |x| Phi(-|x|)
+    const NormalPair n = normal_pair(x);
+    return fma2(n.size, n.tail, make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
+}
+__device__ __forceinline__ float2 gelu_slope_pair(float2 x){             // Phi(x) + x phi(x)
+    const NormalPair n = normal_pair(x);
+    const float2 rest = add2(n.tail, both(1.0f));
+    return fma2(mul2(x, both(0.39894228040143268f)), n.density, make_float2(x.x < 0.0f ? -n.tail.x : rest.x, x.y < 0.0f ? -n.tail.y : rest.y));
 }
 __device__ __forceinline__ float fast_sigmoid(float x){ return __fdividef(1.0f, 1.0f + __expf(-x)); }      // exp(-x) = inf: 1 / inf = 0
 template <int ACT> __device__ __forceinline__ float residual_activation(float x){
-    if constexpr(ACT == B200RL_ACT_GELU) return x * normal_pair(both(x)).phi.x;
+    if constexpr(ACT == B200RL_ACT_GELU) return gelu_pair(both(x)).x;
     else if constexpr(ACT == B200RL_ACT_SILU) return x * fast_sigmoid(x);
     else if constexpr(ACT == B200RL_ACT_SIGMOID) return fast_sigmoid(x);
     else return activation<ACT>(x);
 }
 template <int ACT> __device__ __forceinline__ float residual_d_activation(float x){
-    if constexpr(ACT == B200RL_ACT_GELU){ const NormalPair n = normal_pair(both(x)); return fmaf(x * 0.39894228040143268f, n.density.x, n.phi.x); }
+    if constexpr(ACT == B200RL_ACT_GELU)return gelu_slope_pair(both(x)).x;
     else if constexpr(ACT == B200RL_ACT_SILU){ const float s = fast_sigmoid(x); return s * fmaf(x, 1.0f - s, 1.0f); }
     else if constexpr(ACT == B200RL_ACT_SIGMOID){ const float s = fast_sigmoid(x); return s * (1.0f - s); }
     else return d_activation<ACT>(x);
@@ -106,7 +116,7 @@ template <int ACT> __device__ __forceinline__ void activate8(float (&v)[8]){
     if constexpr(ACT == B200RL_ACT_GELU)
 #pragma unroll
         for(int c = 0; c < 8; c += 2){
-            const float2 x = make_float2(v[c], v[c + 1]), y = mul2(x, normal_pair(x).phi);
+            const float2 y = gelu_pair(make_float2(v[c], v[c + 1]));
             v[c] = y.x; v[c + 1] = y.y;
         }
     else
@@ -117,9 +127,7 @@ template <int ACT> __device__ __forceinline__ void times_slope8(float (&v)[8], c
     if constexpr(ACT == B200RL_ACT_GELU)
 #pragma unroll
         for(int c = 0; c < 8; c += 2){
-            const float2 x = make_float2(at[c], at[c + 1]);
-            const NormalPair n = normal_pair(x);
-            const float2 y = mul2(make_float2(v[c], v[c + 1]), fma2(mul2(x, both(0.39894228040143268f)), n.density, n.phi));
+            const float2 y = mul2(make_float2(v[c], v[c + 1]), gelu_slope_pair(make_float2(at[c], at[c + 1])));
             v[c] = y.x; v[c + 1] = y.y;
         }
     else
@@ -129,7 +137,7 @@ template <int ACT> __device__ __forceinline__ void times_slope8(float (&v)[8], c
 template <int ACT> __device__ __forceinline__ void activate_pairs(float2 (&v)[4]){
 #pragma unroll
     for(int c = 0; c < 4; c++){
-        if constexpr(ACT == B200RL_ACT_GELU) v[c] = mul2(v[c], normal_pair(v[c]).phi);
+        if constexpr(ACT == B200RL_ACT_GELU) v[c] = gelu_pair(v[c]);
         else v[c] = make_float2(residual_activation<ACT>(v[c].x), residual_activation<ACT>(v[c].y));
     }
 }
@@ -137,10 +145,7 @@ template <int ACT> __device__ __forceinline__ void times_slope_pairs(float2 (&v)
 #pragma unroll
     for(int c = 0; c < 4; c++){
         const float2 x = make_float2(at[2 * c], at[2 * c + 1]);
-        if constexpr(ACT == B200RL_ACT_GELU){
-            const NormalPair n = normal_pair(x);
-            v[c] = mul2(v[c], fma2(mul2(x, both(0.39894228040143268f)), n.density, n.phi));
-        }
+        if constexpr(ACT == B200RL_ACT_GELU) v[c] = mul2(v[c], gelu_slope_pair(x));
         else v[c] = mul2(v[c], make_float2(residual_d_activation<ACT>(x.x), residual_d_activation<ACT>(x.y)));
     }
 }

@@ -1,0 +1,52 @@
+"""The residual operators where an absolute bound or an ordinary size sees nothing: activations in their tails, relative to their values; long batches with a remainder, by bounds that a few
+lost rows exceed; the largest sizes that an entry point takes."""
+import math
+
+import pytest
+import torch
+
+from residual_reference import U32, half_step, smallest, act64, assert_within
+
+pytestmark = pytest.mark.gpu
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def every_value(dtype):
+    """All finite numbers of a 16-bit type."""
+    v = torch.arange(65536, device="cuda", dtype=torch.int32).to(torch.int16).view(dtype)
+    return v[torch.isfinite(v)]
+
+
+def gelu_error(x):
+    """Relative error of Phi(-|x|) = P(t) exp(-x^2 / 2), and of the density: 1.2e-5 by the fit of P; its argument t (six roundings), that of P's six additions and products through t^6 (36
+    and 12); the exponential's argument e = x^2 / 2 (a rounding of it is |e| roundings of the result) and the exponential itself, within 2 + 1.2 |e| units of 2^-23."""
+    e = (x * x / 2).clamp(max=100)
+    return 1.2e-5 + 60 * U32 + e * U32 + (2 + 1.2 * e) * 2 * U32
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("few_rows", [True, False])
+def test_gelu_of_every_value_relative_to_its_result(lib, dtype, few_rows):
+    v = every_value(dtype)
+    one = torch.ones(1, 1, device="cuda", dtype=dtype)
+    y = lib.dense_residual_forward(v[:, None], one, "gelu")[1][0] if few_rows else lib.dense_residual_forward(one, v[:, None], "gelu")[1][:, 0]
+    x = v.double()
+    want = act64("gelu", x)
+    # below 2^-126 the exponential may be 0; above the type's largest number nothing is rounded to infinity, since |gelu(x)| <= |x|
+    bound = (half_step(dtype) + 2 * gelu_error(x)) * want.abs() + smallest(dtype) + 2.0 ** -126 * (1 + x.abs()).clamp(max=100)
+    assert_within(y, want, bound, f"gelu {dtype}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("layout", ["rows of one element", "one row"])
+def test_slope_of_gelu_of_every_value_relative_to_its_terms(lib, dtype, layout):
+    v = every_value(dtype)
+    pre = v[:, None].contiguous() if layout == "rows of one element" else v[:v.numel() // 8 * 8].view(1, -1)
+    d = lib.dense_residual_backward_activation(pre, torch.ones_like(pre), "gelu")
+    x = pre.double()
+    phi, along = 0.5 * torch.erfc(-x / math.sqrt(2)), x * torch.exp(-x * x / 2) / math.sqrt(2 * math.pi)
+    along = torch.where(x.abs() > 50, 0 * along, along)
+    terms = 0.5 * torch.erfc(x.abs() / math.sqrt(2)) + along.abs()
+    want = phi + along
+    bound = half_step(dtype) * want.abs() + 2 * gelu_error(x) * terms + 4 * U32 * (phi + along.abs()) + smallest(dtype) + 2.0 ** -126 * (1 + x.abs()).clamp(max=100)
+    assert_within(d, want, bound, f"slope {dtype}")
