@@ -50,3 +50,31 @@ def test_slope_of_gelu_of_every_value_relative_to_its_terms(lib, dtype, layout):
     want = phi + along
     bound = half_step(dtype) * want.abs() + 2 * gelu_error(x) * terms + 4 * U32 * (phi + along.abs()) + smallest(dtype) + 2.0 ** -126 * (1 + x.abs()).clamp(max=100)
     assert_within(d, want, bound, f"slope {dtype}")
+
+
+@pytest.mark.parametrize("layout", [(0, 0), (5, 3)])
+@pytest.mark.parametrize("B, I, O", [(40017, 96, 72), (16400, 72, 300), (4096 + 37, 520, 40), (1000, 30, 50), (577, 200, 260)])
+def test_gradients_of_long_batches_lose_no_row(lib, B, I, O, layout):
+    """Products of one sign, so that a row is a share 1 / B of every sum. A piece of 512 rows is 32 truncating additions of 16 products (and those within each: 40 steps of 2^-23 in all); the
+    pieces, and the shares of the batch that several CTAs take, are added with a rounding each. A column sum is at most B / 64 additions a thread, 8 between threads and those of the shares."""
+    g = torch.Generator(device="cuda").manual_seed(B)
+    draw = lambda n: (torch.rand(B, n + layout[0], device="cuda", generator=g) + 0.5).to(BF16)[:, layout[1]:layout[1] + n]
+    x, d = draw(I), draw(O)
+    d_W, d_b, _ = lib.dense_residual_backward(x.new_zeros(O, I), x, d, want_d_in=False)
+    want, want_b = d.double().t() @ x.double(), d.double().sum(0)
+    pieces, blocks = -(-B // 512), -(-B // 64)
+    bound, bound_b = (2 * 40 + 2 * pieces) * U32, (blocks + 8 + pieces) * U32
+    assert 16 * 0.25 / (B * 2.25) > bound and 16 * 0.5 / (B * 1.5) > bound_b               # the smallest share of 16 rows shows
+    assert_within(d_W, want, bound * want, "d_W")
+    assert_within(d_b, want_b, bound_b * want_b, "d_bias")
+
+
+@pytest.mark.parametrize("B, I, O", [(4096, 256, 200), (5003, 200, 1000), (40017, 96, 72)])
+def test_weight_gradients_have_the_error_of_fp32_sums(lib, B, I, O):
+    """Of products of both signs: a piece's truncations lose half a step of 2^-23 each in the mean, 40 of them of sums no larger than the piece's; what rounds is less. A single accumulator
+    for 4,096 rows would lose eight times that."""
+    g = torch.Generator(device="cuda").manual_seed(B + 1)
+    x, d = (torch.randn(B, n, device="cuda", generator=g).to(BF16) for n in (I, O))
+    d_W = lib.dense_residual_backward(x.new_zeros(O, I), x, d, want_d_in=False)[0]
+    want = d.double().t() @ x.double()
+    assert float((d_W.double() - want).norm() / want.norm()) < (40 + 8) * U32
