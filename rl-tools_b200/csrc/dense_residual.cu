@@ -12,7 +12,7 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const T* d, long long
     float v = 0.0f;
     if(c < cols)
 #pragma unroll 8
-        for(int r = slice; r < rows; r += 32) v += to_float(d[r * ld + c]);
+        for(long long r = slice; r < rows; r += 32) v += to_float(d[r * ld + c]);            // rows may be 2^31 - 1
     shared[slice][lane] = v;
     __syncthreads();
     if(slice || c >= cols) return;

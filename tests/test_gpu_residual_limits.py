@@ -78,3 +78,15 @@ def test_weight_gradients_have_the_error_of_fp32_sums(lib, B, I, O):
     d_W = lib.dense_residual_backward(x.new_zeros(O, I), x, d, want_d_in=False)[0]
     want = d.double().t() @ x.double()
     assert float((d_W.double() - want).norm() / want.norm()) < (40 + 8) * U32
+
+
+def test_bias_gradient_alone_of_the_most_rows_there_can_be(lib):
+    """2^31 - 1 rows, the largest batch of the entry point: a row index of 32 bits would pass its range behind the last one."""
+    B = 2 ** 31 - 1
+    d = torch.zeros(B, 1, device="cuda", dtype=BF16)
+    rows = torch.tensor([0, 31, 32, B // 2, B - 34, B - 32, B - 1], device="cuda")
+    d[rows] = 1.0
+    out = torch.full((1,), 3.0, device="cuda")
+    L, st = lib.lib(), torch.cuda.current_stream().cuda_stream
+    assert L.b200rl_dense_residual_backward_weights(1, None, 0, d.data_ptr(), 1, None, out.data_ptr(), 1, B, 1, 1, None, 0, st) == 0
+    assert out.item() == 3 + rows.numel()
