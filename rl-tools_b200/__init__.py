@@ -48,10 +48,17 @@ class B200RLError(RuntimeError):
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every CUDA source into libb200rl.so for sm_100a (nvcc cross-compiles without a GPU)."""
+    """Compile every CUDA source into libb200rl.so for sm_100a (nvcc cross-compiles without a GPU); then, where torch is installed, the calls on torch tensors."""
+    path = _build_library(force, verbose)
+    import importlib.util
+    if importlib.util.find_spec("torch") is not None:
+        build_tensors(force)
+    return path
+
+
+def _build_library(force, verbose):
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh")] + [os.path.join(ROOT, "include", "b200rl.h"), os.path.abspath(__file__)]
-    build_tensors(force)
     if not force and os.path.exists(LIB_PATH) and all(os.path.getmtime(LIB_PATH) >= os.path.getmtime(d) for d in deps):
         return LIB_PATH
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -86,10 +93,22 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 def build_tensors(force: bool = False) -> str:
     """Compile the calls of the residual operators on torch tensors (host code against torch's headers; it finds the library's entry points at run time)."""
-    src, header = os.path.join(CSRC, "tensors.cpp"), os.path.join(ROOT, "include", "b200rl.h")
-    if not force and os.path.exists(TENSORS_PATH) and all(os.path.getmtime(TENSORS_PATH) >= os.path.getmtime(d) for d in (src, header)):
-        return TENSORS_PATH
+    import importlib.metadata
+    import sys
     import sysconfig
+    src, header = os.path.join(CSRC, "tensors.cpp"), os.path.join(ROOT, "include", "b200rl.h")
+    try:
+        version = importlib.metadata.version("torch")               # without importing it
+    except importlib.metadata.PackageNotFoundError:
+        import torch
+        version = torch.__version__
+    # what a built module goes with besides its sources: it is compiled against one torch and one Python
+    stamp_path, stamp = os.path.join(CSRC, "build", "tensors.txt"), f"torch {version}, Python {sys.version}\n"
+    built = os.path.exists(TENSORS_PATH) and all(os.path.getmtime(TENSORS_PATH) >= os.path.getmtime(d) for d in (src, header))
+    if built and not force and os.path.exists(stamp_path):
+        with open(stamp_path) as f:
+            if f.read() == stamp:
+                return TENSORS_PATH
     import torch
     from torch.utils.cpp_extension import include_paths
     cuda = os.path.dirname(os.path.dirname(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")))
@@ -97,10 +116,16 @@ def build_tensors(force: bool = False) -> str:
     cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
     cmd += ["-isystem" + d for d in include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include")]]
     cmd += [src, "-o", tmp, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise B200RLError(f"the calls on torch tensors need a C++ compiler ({e}); the C library itself is built") from None
     if res.returncode != 0:
         raise B200RLError("g++ failed on " + src + ":\n" + res.stdout + res.stderr)
+    os.makedirs(os.path.dirname(stamp_path), exist_ok=True)
     os.replace(tmp, TENSORS_PATH)
+    with open(stamp_path, "w") as f:
+        f.write(stamp)
     return TENSORS_PATH
 
 
