@@ -30,8 +30,8 @@ static int dispatch_row(int dim, F f){
     if(dim <= 2048) return f(Shape<256, 8>{});
     return dim <= 4096 ? f(Shape<512, 8>{}) : f(Shape<1024, 8>{});
 }
-// CTAs of the backward pass on a multiprocessor, which leaves a thread 64 to 168 registers
-template <typename T> __host__ __device__ constexpr int backward_ctas(int tpr, int e){
+// CTAs of the backward pass on a multiprocessor that leave a thread 64 to 168 registers
+template <typename T> constexpr int backward_ctas(int tpr, int e){
     const bool narrow = sizeof(T) == 2;
     return tpr == 32 ? (narrow && e == 8 ? 5 : 3) : tpr == 128 ? (narrow && e == 8 ? 5 : 4) : tpr == 256 ? 2 : 1;
 }
@@ -317,8 +317,15 @@ template <int TPR, int E, bool BIAS, bool GATE> struct Kept {
     float4* mine;                                            // [COUNT][E / 4][TPR]
     __device__ __forceinline__ float4& at(int array, int quad){ return mine[(array * (E / 4) + quad) * TPR]; }
 };
+// CTAs that are resident at once, their shared memory counted too: what they keep, the exchanges' buffers, 1 KB that each costs besides. Only 16-bit rows of 1025 to 2048 elements with
+// biases and a gate are held to fewer by it (three instead of four: 16384 x 2048 with a gate per channel 129 us, planned and compiled for four 209).
+template <typename T, int TPR, int E, bool BIAS, bool GATE> constexpr int backward_resident(){
+    constexpr int bytes = (TPR < 128 ? 128 / TPR : 1) * Kept<TPR, E, BIAS, GATE>::worker_bytes + 2 * 4 * (TPR / 32) * 4 + 16 + 1024, fit = 228 * 1024 / bytes;
+    static_assert(fit >= 1);
+    return fit < backward_ctas<T>(TPR, E) ? fit : backward_ctas<T>(TPR, E);
+}
 template <typename T, int VEC, int TPR, int E, bool BIAS, bool GATE>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, backward_ctas<T>(TPR, E)) norm_backward_kernel(NormBackward a){
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, backward_resident<T, TPR, E, BIAS, GATE>()) norm_backward_kernel(NormBackward a){
     constexpr int WORKERS = TPR < 128 ? 128 / TPR : 1, P = E / 2;
     using R = Row<T, VEC, TPR, E>;
     using K = Kept<TPR, E, BIAS, GATE>;
@@ -570,10 +577,15 @@ __global__ void __launch_bounds__(512) norm_backward_sums_kernel(NormBackward a,
     else static_cast<T*>(a.d_gate)[g.group * a.lddg + c] = from_float<T>(v);
 }
 
-// Workers of the backward pass, and the consecutive rows that each takes: as many as are resident at once, a row each where there are fewer rows than that.
+// Workers of the backward pass, and the consecutive rows that each takes: as many as are resident at once, a row each where there are fewer rows than that. `whole`: the form with biases
+// and gate, of which fewer may be.
 template <typename T>
-static void plan_workers(int rows, int dim, int* workers, int* rows_per_worker){
-    const int most = dispatch_row<T>(dim, [](auto shape){ return NUM_SMS * backward_ctas<T>(decltype(shape)::tpr, decltype(shape)::e) * (decltype(shape)::tpr == 32 ? 4 : 1); });
+static void plan_workers(int rows, int dim, bool whole, int* workers, int* rows_per_worker){
+    const int most = dispatch_row<T>(dim, [&](auto shape){
+        constexpr int TPR = decltype(shape)::tpr, E = decltype(shape)::e, all = backward_resident<T, TPR, E, true, true>(), less = backward_resident<T, TPR, E, false, false>();
+        static_assert(backward_resident<T, TPR, E, true, false>() == less && backward_resident<T, TPR, E, false, true>() == less);
+        return NUM_SMS * (whole ? all : less) * (TPR == 32 ? 4 : 1);
+    });
     *rows_per_worker = (rows - 1) / most + 1;
     *workers = (rows - 1) / *rows_per_worker + 1;
 }
@@ -649,8 +661,8 @@ int b200rl_norm_residual_forward(int type, int post, const float* post_weight, c
 size_t b200rl_norm_residual_backward_scratch_bytes(int rows, int dim){
     if(rows < 1 || dim < 1 || dim > B200RL_NORM_MAX_DIM) return 0;
     int workers, workers32, per;
-    plan_workers<__half>(rows, dim, &workers, &per);
-    plan_workers<float>(rows, dim, &workers32, &per);
+    plan_workers<__half>(rows, dim, false, &workers, &per);          // enough for the other form too, which has no more workers
+    plan_workers<float>(rows, dim, false, &workers32, &per);
     return (size_t)(workers > workers32 ? workers : workers32) * (SUMS + 2) * dim * sizeof(float);
 }
 
@@ -681,9 +693,6 @@ int b200rl_norm_residual_backward(int type, int post, const float* post_weight, 
     NormBackward a{branch, row_pitch(ldb, rows, dim), gate, row_pitch(ldg, gates, dim), gate_rows, out, row_pitch(ldo, rows, dim), d_out, row_pitch(lddo, rows, dim),
                    d_normed, row_pitch(lddn, rows, dim), d_branch, row_pitch(lddb, rows, dim), d_residual, row_pitch(lddr, rows, dim), d_gate, row_pitch(lddg, gates, dim),
                    post_weight, post_bias, pre_weight, {d_post_weight, d_post_bias, d_pre_weight, d_pre_bias}};
-    if(type == B200RL_TYPE_FLOAT32) plan_workers<float>(rows, dim, &a.workers, &a.rows_per_worker); else plan_workers<__half>(rows, dim, &a.workers, &a.rows_per_worker);
-    a.partials = static_cast<float*>(scratch);
-    a.pieces = a.partials + (size_t)SUMS * a.workers * dim;
     a.post = post; a.pre = pre; a.rows = rows; a.dim = dim; a.accumulate = accumulate; a.scale = scale; a.epsilon = epsilon;
     const int n = 16 / (int)e;
     const bool vector = dim % n == 0 && (!branch || rows_aligned(branch, a.ldb, e)) && (!gate || rows_aligned(gate, a.ldg, e)) && (pre == B200RL_NORM_NONE || rows_aligned(out, a.ldo, e)) &&
@@ -691,6 +700,10 @@ int b200rl_norm_residual_backward(int type, int post, const float* post_weight, 
                         (!d_residual || rows_aligned(d_residual, a.lddr, e)) && (!d_gate || rows_aligned(d_gate, a.lddg, e));
     for(int i = 0; i < SUMS; i++) if(a.d_params[i]) a.sums[a.n_sums++] = i;
     const bool bias = d_post_bias || d_pre_bias || (post_bias && gate);
+    const bool whole = !vector || (bias && gate);
+    if(type == B200RL_TYPE_FLOAT32) plan_workers<float>(rows, dim, whole, &a.workers, &a.rows_per_worker); else plan_workers<__half>(rows, dim, whole, &a.workers, &a.rows_per_worker);
+    a.partials = static_cast<float*>(scratch);
+    a.pieces = a.partials + (size_t)SUMS * a.workers * dim;
     int rc = B200RL_ERR_UNSUPPORTED;
     B200RL_DISPATCH_TYPE(type, rc = dispatch_row<T>(dim, [&](auto shape){
         constexpr int TPR = decltype(shape)::tpr, E = decltype(shape)::e, V = 16 / sizeof(T);
