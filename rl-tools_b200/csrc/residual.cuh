@@ -112,28 +112,6 @@ template <int ACT> __device__ __forceinline__ float residual_d_activation(float 
     else return d_activation<ACT>(x);
 }
 // eight values in place; eight values times the slopes at eight places
-template <int ACT> __device__ __forceinline__ void activate8(float (&v)[8]){
-    if constexpr(ACT == B200RL_ACT_GELU)
-#pragma unroll
-        for(int c = 0; c < 8; c += 2){
-            const float2 y = gelu_pair(make_float2(v[c], v[c + 1]));
-            v[c] = y.x; v[c + 1] = y.y;
-        }
-    else
-#pragma unroll
-        for(int c = 0; c < 8; c++) v[c] = residual_activation<ACT>(v[c]);
-}
-template <int ACT> __device__ __forceinline__ void times_slope8(float (&v)[8], const float (&at)[8]){
-    if constexpr(ACT == B200RL_ACT_GELU)
-#pragma unroll
-        for(int c = 0; c < 8; c += 2){
-            const float2 y = mul2(make_float2(v[c], v[c + 1]), gelu_slope_pair(make_float2(at[c], at[c + 1])));
-            v[c] = y.x; v[c + 1] = y.y;
-        }
-    else
-#pragma unroll
-        for(int c = 0; c < 8; c++) v[c] *= residual_d_activation<ACT>(at[c]);
-}
 template <int ACT> __device__ __forceinline__ void activate_pairs(float2 (&v)[4]){
 #pragma unroll
     for(int c = 0; c < 4; c++){

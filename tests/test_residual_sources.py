@@ -26,3 +26,11 @@ def test_no_load_may_pass_the_wait_for_the_kernel_before(name):
 def test_no_register_of_a_tensor_memory_load_is_named_before_its_wait():
     """What tcgen05.ld writes is there behind tcgen05.wait::ld alone. With both in one statement no copy, spill or loop variable of the registers can lie between them."""
     assert not re.findall(r"tmem_ld_32x32|tmem_wait_ld|tcgen05\.ld", code("product_tc.cu"))
+
+
+def test_every_function_of_these_sources_is_called():
+    text = {name: code(name) for name in SOURCES + ["tcgen05.cuh"]}
+    everything = "\n".join(text.values())
+    defined = {m for name in SOURCES for m in re.findall(r"__device__ __forceinline__ [\w:<> ,]+?[ &*](\w+)\(", text[name])}
+    assert len(defined) > 40
+    assert [f for f in sorted(defined) if len(re.findall(rf"\b{f}\b", everything)) < 2] == []
