@@ -23,12 +23,17 @@ template <int TPR, int E> struct Shape { static constexpr int tpr = TPR, e = E; 
 template <typename T, typename F>
 static int dispatch_row(int dim, F f){
     if(dim <= 256) return f(Shape<32, 8>{});
-    if constexpr(sizeof(T) == 2) if(dim <= 512) return f(Shape<32, 16>{});
-    if(dim <= 1024) return f(Shape<128, 8>{});
-    if constexpr(sizeof(T) == 2) if(dim <= 2048) return f(Shape<128, 16>{});
-    if constexpr(sizeof(T) == 2) return dim <= 4096 ? f(Shape<256, 16>{}) : f(Shape<512, 16>{});
-    if(dim <= 2048) return f(Shape<256, 8>{});
-    return dim <= 4096 ? f(Shape<512, 8>{}) : f(Shape<1024, 8>{});
+    if constexpr(sizeof(T) == 2){
+        if(dim <= 512) return f(Shape<32, 16>{});
+        if(dim <= 1024) return f(Shape<128, 8>{});
+        if(dim <= 2048) return f(Shape<128, 16>{});
+        return dim <= 4096 ? f(Shape<256, 16>{}) : f(Shape<512, 16>{});
+    }
+    else{
+        if(dim <= 1024) return f(Shape<128, 8>{});
+        if(dim <= 2048) return f(Shape<256, 8>{});
+        return dim <= 4096 ? f(Shape<512, 8>{}) : f(Shape<1024, 8>{});
+    }
 }
 // CTAs of the backward pass on a multiprocessor that leave a thread 64 to 168 registers
 template <typename T> constexpr int backward_ctas(int tpr, int e){

@@ -34,3 +34,14 @@ def test_every_function_of_these_sources_is_called():
     defined = {m for name in SOURCES for m in re.findall(r"__device__ __forceinline__ [\w:<> ,]+?[ &*](\w+)\(", text[name])}
     assert len(defined) > 40
     assert [f for f in sorted(defined) if len(re.findall(rf"\b{f}\b", everything)) < 2] == []
+
+
+def test_the_norms_are_built_for_the_row_shapes_of_their_types_alone(lib):
+    """The threads of a row and the elements of a thread: 16-bit rows take up to 16 elements a thread, fp32 rows 8."""
+    import subprocess
+    names = subprocess.run(["nm", "-C", lib.LIB_PATH], capture_output=True, text=True, check=True).stdout
+    built = {}
+    for kernel, of, threads, elements in re.findall(r"b200rl::norm_(forward|backward)_kernel<([\w ]+), \d+, (\d+), (\d+)", names):
+        built.setdefault((kernel, of), set()).add((int(threads), int(elements)))
+    narrow, wide = {(32, 8), (32, 16), (128, 8), (128, 16), (256, 16), (512, 16)}, {(32, 8), (128, 8), (256, 8), (512, 8), (1024, 8)}
+    assert built == {(kernel, of): wide if of == "float" else narrow for kernel in ("forward", "backward") for of in ("float", "__half", "__nv_bfloat16")}
