@@ -231,8 +231,9 @@ PyObject* dense_residual_backward(PyObject* const* a){
 
 int64_t gate_count(const char* call, const at::Tensor* gate, long long gate_rows, int64_t rows){
     if(!gate) return 0;
+    if(rows == 0) return gate->dim() == 2 ? gate->size(0) : 0;      // no row looks at it
     if(gate_rows < 1 || gate_rows > INT_MAX) refuse(call, ": a gate row serves at least one row");
-    return rows == 0 ? 0 : (rows - 1) / gate_rows + 1;
+    return (rows - 1) / gate_rows + 1;
 }
 void check_dim(const char* call, int64_t D){
     if(D < 1 || D > B200RL_NORM_MAX_DIM) refuse(call, ": rows have 1 to ", B200RL_NORM_MAX_DIM, " elements, not ", D);
@@ -310,6 +311,7 @@ PyObject* norm_residual_backward(PyObject* const* a){
     void *stream = o.here(), *ws;
     const size_t n = E.norm_residual_backward_scratch_bytes((int)R, (int)D);
     const at::Tensor keep = workspace(n, *first, &ws);
+    if(R == 0 && d_gate.get()) d_gate.get()->zero_();               // sums over no rows; the C call takes a gate of an empty batch to have none
     check(E.norm_residual_backward(o.type, post, p[0], p[1], mb.p, mb.ld, mg.p, mg.ld, (int)gate_rows, scale, mo.p, mo.ld, pre, p[2], mdo.p, mdo.ld, mdn.p, mdn.ld, mdb.p, mdb.ld, mdr.p,
                                    mdr.ld, mdg.p, mdg.ld, g[0], g[1], g[2], g[3], given, (int)R, (int)D, epsilon, ws, n, stream));
     return Py_BuildValue("{sNsNsNsNsNsNsN}", "d_branch", d_branch.hand(), "d_residual", d_residual.hand(), "d_gate", d_gate.hand(), gradient[0], d_param[0].hand(), gradient[1],

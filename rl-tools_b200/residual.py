@@ -81,7 +81,7 @@ def dense_residual_backward(W, x, d_pre, d_W=None, d_bias=None, add=None, pre_in
 def norm_residual_forward(branch, residual, post="none", post_weight=None, post_bias=None, gate=None, gate_rows=1, scale=1.0, pre="none", pre_weight=None, pre_bias=None,
                           epsilon=1e-5, out=None, normed=None):
     """out = residual + scale gate post(branch), normed = pre(out); returns (out, normed or None). post, pre: "none", "layer" or "rms", each with its weight and bias. gate
-    [ceil(rows / gate_rows), dim]: row r takes gate row r // gate_rows. branch or residual may be None; out may be the residual itself."""
+    [ceil(rows / gate_rows), dim]: row r takes gate row r // gate_rows (a batch without rows takes any gate). branch or residual may be None; out may be the residual itself."""
     T = _module or _tensors()
     try:
         return T.norm_residual_forward(branch, residual, NORM.get(post, post), post_weight, post_bias, gate, gate_rows, scale, NORM.get(pre, pre), pre_weight, pre_bias, epsilon, out,
