@@ -6,6 +6,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include "../../include/b200rl.h"
 #include <string>
@@ -348,7 +349,7 @@ template <PyObject* (*F)(PyObject* const*), int N> PyObject* guarded(PyObject*, 
     try { return F(args); }
     catch(const Refusal& r){ PyErr_SetString(g_refusal, r.what.c_str()); }
     catch(const Status& s){ PyErr_SetObject(g_status, PyLong_FromLong(s.status)); }
-    catch(const std::exception& e){ PyErr_SetString(PyExc_RuntimeError, e.what()); }
+    catch(...){ torch::translate_exception_to_python(std::current_exception()); }       // torch's own: out of memory stays torch.OutOfMemoryError
     return nullptr;
 }
 

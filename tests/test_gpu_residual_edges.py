@@ -31,3 +31,12 @@ def test_gradients_of_a_batch_without_rows(lib):
     given, weight = torch.full((1, 24), 5.0, device="cuda", dtype=BF16), torch.full((24,), 5.0, device="cuda")
     lib.norm_residual_backward(x, out, d_out=x, d_normed=x, **norms, pre="layer", d_gate=given, d_post_weight=weight)
     assert not given.any() and (weight == 5).all()                  # a gate's gradient is overwritten, a parameter's accumulated onto
+
+
+@pytest.mark.gpu
+def test_outputs_that_no_memory_holds_raise_what_torch_raises(lib):
+    """320 GB of outputs from operands of 0.8 MB: refused by the allocator, as the error that programs catch to take a smaller batch."""
+    x = torch.zeros(400000, 1, device="cuda", dtype=BF16)
+    with pytest.raises(torch.OutOfMemoryError):
+        lib.dense_residual_forward(x, x, "identity")
+    assert lib.dense_residual_forward(x[:5], x[:40], "identity")[1].shape == (40, 5)
