@@ -244,14 +244,16 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_forward_kernel(Nor
 #pragma unroll
     for(int k = 0; k < 4; k++) if(parameters[k]) place[k] = n++; else place[k] = -1;
     auto kept = [&](int k, int i) -> float4& { return kept_memory[((place[k] * ROWS + threadIdx.x / TPR) * (E / 4) + i) * TPR + threadIdx.x % TPR]; };
+    {
+        float p[4][E];                                                   // all loads under way before the first is put away
 #pragma unroll
-    for(int k = 0; k < 4; k++)
-        if(parameters[k]){
-            float p[E];
-            row.parameters(parameters[k], 0.0f, p);
+        for(int k = 0; k < 4; k++) if(parameters[k]) row.parameters(parameters[k], 0.0f, p[k]);
 #pragma unroll
-            for(int i = 0; i < E / 4; i++) kept(k, i) = make_float4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
-        }
+        for(int k = 0; k < 4; k++)
+            if(parameters[k])
+#pragma unroll
+                for(int i = 0; i < E / 4; i++) kept(k, i) = make_float4(p[k][4 * i], p[k][4 * i + 1], p[k][4 * i + 2], p[k][4 * i + 3]);
+    }
     auto affine = [&](float2 (&v)[P], int weight, int bias){
         if(parameters[weight])
 #pragma unroll
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, backward_resident<T, TP
             if constexpr(BIAS){
                 if(a.d_gate){
                     float b[E];
-                    if(post) row.parameters(a.post_bias, 0.0f, b);
+                    if(post) row.parameters(opaque(a.post_bias), 0.0f, b);      // asked for with every row: kept over the rows it takes registers that lead to spills
 #pragma unroll
                     for(int i = 0; i < E / 4; i++){
                         float2 v0 = u[2 * i], v1 = u[2 * i + 1];
