@@ -663,9 +663,11 @@ int b200rl_shuffle_rows(float* data, int ld, int n_rows, unsigned long long colu
  *     lie in the arenas of b200rl_adam_step; 16-bit weights are the caller's copy of its fp32 master weights.
  *   - row pitches (ld*) are in elements of `type` and at least the row's length; rows may start at any address that is a multiple of the
  *     element's size (fastest: 16-byte aligned rows). A pitch of a matrix with at most one row is not looked at.
- *   - sums, statistics and products are held in fp32 and rounded to `type` once, when they are stored.
+ *   - sums, statistics and products are held in fp32 and rounded to `type` once, when they are stored. The tensor cores truncate where they add: a
+ *     product's sums of one sign are short by 2e-5 of themselves over 16,384 terms, 5e-5 over 65,536 and 8e-4 over a million (half a step of
+ *     float16 is 5e-4, of bfloat16 4e-3). Weight gradients are not, see there.
  *   - calls that share scratch, a workspace or a gradient must be ordered on one stream (or by events).
- *   - an output may not overlap an input, unless a comment below allows it.
+ *   - an output may not overlap an input, unless a comment below allows it, nor another output.
  * ------------------------------------------------------------------------------------------------------- */
 #define B200RL_TYPE_FLOAT32 0
 #define B200RL_TYPE_BFLOAT16 1

@@ -3,9 +3,11 @@
 // and its gradients. Memory-bound: forward reads branch and residual and writes out and normed, backward reads out, d_normed, d_out and branch and writes
 // d_residual and d_branch, each once. A row is held in the registers of 32 to 1,024 threads as fp32, so the two passes of a variance (mean, then squared deviations)
 // cost no second read. The statistics are not stored for the backward pass: it holds the rows in registers anyway and computes them again.
-// Measured, 16384 x 4096 bfloat16, root-mean-square norms on both sides: forward with a gate per channel 90 us (6 TB/s), gradients 159 us with that gate, 142 us without
-// one (5.7 TB/s; 537 and 805 MB cannot be avoided). The forward pass is bound by memory; the gradients by issue (half of all cycles, eight or sixteen warps resident that meet three
-// times a row). One row of 4096: 2.9 and 7 us, the launches and a chain of barriers. Before rows were fetched ahead and parameters kept in shared memory: 154 and 404 us.
+// Measured, 16384 x 4096 bfloat16, calls in a graph: root-mean-square norms on both sides, forward 89 us without a gate, 90 with one per channel (5.9 TB/s), 102 with one per element;
+// gradients 143, 161 and 200 us (5.6, 5.0 and 5.3 TB/s; 537 and 805 MB cannot be avoided, a gate per element is 134 and 268 more). Layer norms with biases and a gate per channel 122 and 347.
+// The forward pass is bound by memory; the gradients by issue (half of all cycles, eight or sixteen warps resident that meet three times a row), with biases and a gate by the shared
+// memory that holds seven values a column too. One row of 4096: 2.6 and 6.6 us, the launches and a chain of barriers. Before rows were fetched ahead and parameters kept in
+// shared memory: 154 and 404 us.
 #include "residual.cuh"
 #include <atomic>
 #include <type_traits>

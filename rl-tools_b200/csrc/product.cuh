@@ -25,7 +25,7 @@ struct Product {
     float* row_sums;                            // EPI_SUM: (+)= sum_k A(m, k), or NULL
 };
 
-// bytes of workspace for this product on the tensor cores: partial sums where k is split, copies of operands (and of fp32 results) that TMA cannot address
+// bytes of workspace for this product on the tensor cores: partial sums where k is split, copies of operands that TMA cannot address
 size_t product_tc_workspace_bytes(const Product& g, int epilogue);
 int product_tc(const Product& g, int type, int epilogue, void* workspace, size_t workspace_bytes, cudaStream_t s);
 // the forward product of a few rows, without a workspace

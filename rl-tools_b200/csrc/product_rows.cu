@@ -3,7 +3,7 @@
 // eighth block of 32 k; W is the left operand of mma.sync (16 of its rows x 16 k), the rows of x the right one (8 at a time). Which k an instruction's slots stand for does not
 // matter as long as both operands agree, so a lane loads eight consecutive k of its rows by one 16-byte access and feeds two instructions with them. The eight warps' sums meet in
 // shared memory, in their order, and the layer's epilogue follows.
-// Measured (bfloat16, 1024 -> 4096): 1 row 3.1 us, 16 rows 3.3 us, 32 rows 4.8 us (64 would be 7.5), where W's 8.4 MB take 1.3 us at the rate of memory and a launch about 2; the
+// Measured (bfloat16, 1024 -> 4096, calls in a graph): 1 row 3.2 us, 16 rows 3.5 us, 32 rows 4.9 us (64 would be 7.5; the library's product takes 5, 3.7 and 3.8), where W's 8.4 MB take 1.3 us at the rate of memory and a launch about 2; the
 // tensor-memory kernel takes 8.5 us.
 #include "product.cuh"
 #include <limits.h>

@@ -10,10 +10,15 @@
 // 1e-4); pieces of 32 additions are added in registers with rounding, while the next piece runs. Error of a weight gradient over 4,096 rows: 4.8e-7 (2-norm), an fp32 loop's 6.1e-7.
 // Products of few tiles share each tile's k among the CTAs of a cluster, which add up through one another's shared memory.
 //
-// Bound by the tensor cores where the products are long: 16384 x 4096 x 4096 bfloat16 336 us = 1,637 TFLOP/s (the tensor pipe busy 84 to 92% of the cycles; the same product
-// in the library's form takes 340 to 348), 4096 x 1024 x 4096 26 us, with gelu and pre-activations kept 34. A stage's operands take 64 bytes a cycle and multiprocessor from L2, all
-// that it gives; tiles of 256 x 256 over a pair are what the tensor memory holds twice (128 x 128 by one CTA: 740 us). Small products are bound by the way through the kernel
-// (256 x 256 x 256 4.5 us: 0.9 until the first operands are there, 1 for the products, 0.8 for the epilogue, the rest launch).
+// Bound by the tensor cores where the products are long: the tensor pipe is busy 91% of the cycles at 8192 x 4096 x 4096. A stage's operands would have to come from L2 at 64 bytes a
+// cycle and multiprocessor to keep it busy all the time; so they come at 58. Tiles of 256 x 256 over a pair are what the tensor memory holds twice (128 x 128 by one CTA: 740 us for
+// 16384 x 4096 x 4096). Small products are bound by the way through the kernel (256 x 256 x 256: 0.9 us until the first operands are there, 1 for the products, 0.8 for the epilogue, the
+// rest launch). us of one bfloat16 product, calls in a graph with inputs that stay, and in brackets the library's product on the same box:
+//   16384 x 4096 x 4096  forward 331 (334), gradient of the input 328 (333), of the weights 391 (374)
+//   4096 x 1024 x 4096   26 (29), 27 (25), 34 (26); forward with bias, gelu, residual and pre-activations 38, gradient of the input with gelu's slope and an addend 31
+//   2048 x 2048 x 2048   17 (14), 16 (14), 18 (14)
+//   1024 x 1024 x 1024   7.8 (4.9), 7.5 (4.8), 7.9 (4.7)
+//   256 x 256 x 256      4.4 (2.7), 4.1 (2.7), 4.4 (2.7)
 #include "product.cuh"
 #include "tcgen05.cuh"
 #include <cuda.h>
@@ -750,8 +755,8 @@ static long long matrix_cols(const Operand& o, int r, int k){ return o.k_rows ? 
 static TcPlan plan_product(const Product& g, int epilogue){
     TcPlan p{};
     const int k_blocks = (g.k - 1) / KB + 1;
-    // Shape of the tiles and shares of k, by the cycles that a CTA needs: for a block of 64 k the bytes of its stage at the 48 a cycle that L2 gives a multiprocessor when all ask
-    // (measured; the MMAs take 128 to 512), for a tile 1,500 until its sums are out, for a shared tile 1,500 and 1,000 a share more. Sharing a tile needs a CTA for each share at the
+    // Shape of the tiles and shares of k, by the cycles that a CTA needs: for a block of 64 k the bytes of its stage at 48 a cycle, what L2 gives a multiprocessor in short
+    // products, which the rule is for (long ones of pairs get 58; the MMAs take 128 to 512), for a tile 1,500 until its sums are out, for a shared tile 1,500 and 1,000 a share more. Sharing a tile needs a CTA for each share at the
     // same time. us by tiles of 64 / 128 / 256 columns (* the rule's choice): 1024 x 1024 x 1024 7.8* / 8.9 / 7.7, 128 x 4096 x 4096 13.8 / 12.0* / 16.6, 2048 x 2048 x 2048
     // 37.5 / 23.2 / 16.4*, 4096 x 512 x 512 8.2 / 6.8* / 6.9, 512 x 1024 x 1024 7.6* / 8.7 / 7.6.
     if(g.m > INT_MAX - 1024 || g.n > INT_MAX - 1024 || g.k > INT_MAX - 1024) return p;

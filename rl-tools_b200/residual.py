@@ -4,7 +4,8 @@ the norms around a block with its gate and residual scale, and dropout whose mas
 Matrices are 2-D tensors of one type (bfloat16 or float16; the norms and dropout take float32 too) whose rows may be views into wider tables; biases, norm weights
 and every parameter gradient are float32, so that they can be slices of the arenas that b200rl_adam_step steps. A gradient that is passed in is
 accumulated onto, one that is not is made. What is passed has to lie on the current device; calls run on its current stream. Arguments that no kernel
-takes raise B200RLError. One block, forward and backward (x the residual stream, n = pre(x) from the block before):
+takes raise B200RLError. The calls take no part in autograd: operands that require gradients are taken as they are, results carry none, and writing into a tensor that was passed
+does not raise its version; the gradients are the calls below. One block, forward and backward (x the residual stream, n = pre(x) from the block before):
 
     h_pre, h = dense_residual_forward(W1, n, "gelu", bias=b1, want_pre=True)
     _, f     = dense_residual_forward(W2, h, "identity", bias=b2)
