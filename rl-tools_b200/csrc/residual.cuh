@@ -72,14 +72,15 @@ __device__ __forceinline__ float across(float2 v){ return v.x + v.y; }
 // The normal distribution: Phi(-|x|) = exp(-x^2 / 2) P(t), t = 1 / (1 + c z), z = |x| / sqrt 2, with P(t) = t (b1 + t (b2 + ... t b6)) in place of exp(z^2) erfc(z) / 2. P and c are the
 // minimax fit of this form over 0 <= z <= 9.4, by linear programming on the relative error weighted by max(erfc(z), 1/30): off by 4e-7 of the value at 0, by at most 1.2e-5 of it
 // in the tail, where the values themselves vanish, a three-hundredth of half a step of bfloat16 and a fortieth of float16's, whatever x is. (Nothing is subtracted from 1 for
-// x < 0: it would leave nothing of the tail.) Two at a time; the two reciprocals are one, of the product (|x| is cut at 20, where the density has long been 0).
+// x < 0: it would leave nothing of the tail.) Two at a time (|x| is cut at 20, where the density has long been 0), each
+// with a reciprocal of its own: one for both, of the product, takes 0.7% off 4096 x 1024 x 4096 and makes the last bit of a result depend on its neighbour, which behind the last of an
+// odd number of rows is whatever a register holds.
 struct NormalPair { float2 size, tail, density; };                       // |x| up to 20, -Phi(-|x|), exp(-x^2 / 2)
 __device__ __forceinline__ NormalPair normal_pair(float2 x){
     NormalPair n;
     n.size = make_float2(fminf(fabsf(x.x), 20.0f), fminf(fabsf(x.y), 20.0f));
     const float2 d = fma2(n.size, both(0.42263395f * 0.70710678118654752f), both(1.0f));
-    const float r = __fdividef(1.0f, d.x * d.y);
-    const float2 t = mul2(make_float2(d.y, d.x), both(r));
+    const float2 t = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
     const float2 e = mul2(mul2(x, x), both(-0.5f));
     n.density = make_float2(__expf(e.x), __expf(e.y));
     float2 p = fma2(t, both(0.0805534029f), both(-0.229271916f));

@@ -90,3 +90,28 @@ def test_bias_gradient_alone_of_the_most_rows_there_can_be(lib):
     L, st = lib.lib(), torch.cuda.current_stream().cuda_stream
     assert L.b200rl_dense_residual_backward_weights(1, None, 0, d.data_ptr(), 1, None, out.data_ptr(), 1, B, 1, 1, None, 0, st) == 0
     assert out.item() == 3 + rows.numel()
+
+
+@pytest.mark.parametrize("act", ["relu", "tanh", "fast_tanh", "sigmoid", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_an_activation_is_a_function_of_its_element_alone(lib, dtype, act):
+    """Whatever stands beside a value, in its row or in the rows before and behind it, and whichever kernel takes it, the result has the same bits: a row of a batch is what it is alone."""
+    v = every_value(dtype)
+    v = v[:v.numel() // 8 * 8]
+    n, one = v.numel(), torch.ones(1, 1, device="cuda", dtype=dtype)
+    y = lib.dense_residual_forward(v[:, None], one, act)[1][0]                                # a few rows: element by element
+    slope = lib.dense_residual_backward_activation(v[:, None].contiguous(), torch.ones(n, 1, device="cuda", dtype=dtype), act)[:, 0]
+    assert torch.equal(lib.dense_residual_backward_activation(v[None], torch.ones(1, n, device="cuda", dtype=dtype), act)[0].nan_to_num(7.0), slope.nan_to_num(7.0))
+    same = lambda a, b, what: torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) or pytest.fail(f"{what}: {int((a.nan_to_num(7.0) != b.nan_to_num(7.0)).sum())} of {n} values differ")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for _ in range(3):
+        p = torch.randperm(n, device="cuda", generator=g)
+        w = v[p]
+        # rows of one element (2-byte accesses) and of 64 (16-byte accesses)
+        same(lib.dense_residual_forward(one, w[:, None], act)[1][:, 0], y[p], "forward, rows of one")
+        eye = torch.eye(64, device="cuda", dtype=dtype)
+        finite = torch.where(w.abs() < 1e30, w, torch.zeros_like(w)) if dtype == BF16 else w  # a product with 0 would spread what overflows
+        wide, keep = finite[:n // 64 * 64].view(-1, 64), (finite == w)[:n // 64 * 64]
+        same(torch.where(keep, lib.dense_residual_forward(eye, wide, act)[1].reshape(-1), y[p][:keep.numel()]), y[p][:keep.numel()], "forward, rows of 64")
+        same(lib.dense_residual_backward(one, None, torch.ones(n, 1, device="cuda", dtype=dtype), pre_in=w[:, None].contiguous(), act_in=act, want_grads=False)[2][:, 0], slope[p], "slope, rows of one")
+        same(lib.dense_residual_backward(torch.ones(1, n, device="cuda", dtype=dtype), None, one, pre_in=w[None], act_in=act, want_grads=False)[2][0], slope[p], "slope, one row")
