@@ -15,7 +15,7 @@
 // 16384 x 4096 x 4096). Small products are bound by the way through the kernel (256 x 256 x 256: 0.9 us until the first operands are there, 1 for the products, 0.8 for the epilogue, the
 // rest launch). us of one bfloat16 product, calls in a graph with inputs that stay, and in brackets the library's product on the same box:
 //   16384 x 4096 x 4096  forward 331 (334), gradient of the input 328 (333), of the weights 391 (374)
-//   4096 x 1024 x 4096   26 (29), 27 (25), 34 (26); forward with bias, gelu, residual and pre-activations 38, gradient of the input with gelu's slope and an addend 31
+//   4096 x 1024 x 4096   26 (29), 27 (25), 34 (26); forward with bias, gelu, residual and pre-activations 39, gradient of the input with gelu's slope and an addend 31
 //   2048 x 2048 x 2048   17 (14), 16 (14), 18 (14)
 //   1024 x 1024 x 1024   7.8 (4.9), 7.5 (4.8), 7.9 (4.7)
 //   256 x 256 x 256      4.4 (2.7), 4.1 (2.7), 4.4 (2.7)
